@@ -1,4 +1,4 @@
-"""ctypes binding of lib/libschemanet_hip.so (C ABI: include/schemanet_hip.h).
+"""ctypes binding of lib/libschemanet_hip.so (C ABI: include/schemanet_hip.h and include/schemanet_blocks.h).
 
 This is the only place the product touches native code.  There is NO CPU fallback: if the
 library is missing or no MI355X is visible, every entry point raises RuntimeError.
@@ -69,6 +69,24 @@ class GraphArgs(_SizedArgs):
         ("out_n", c_void_p), ("out_n_max", c_void_p), ("attn_cls_masked", c_void_p),
         ("skip_edge_padding", c_int),
         ("rerank", POINTER(RerankArgs)),
+    ]
+
+
+class BlockNormsArgs(_SizedArgs):
+    """struct sn_block_norms_args (include/schemanet_blocks.h)."""
+    _fields_ = [
+        ("struct_size", c_uint32), ("dtype", c_int32), ("param_dtype", c_int32), ("rms", c_int32),
+        ("rows", c_int64), ("width", c_int32), ("rows_per_graph", c_int32), ("n_valid", c_void_p),
+        ("eps", c_float), ("has_post", c_int32), ("has_pre", c_int32),
+        ("x", c_void_p), ("branch", c_void_p), ("gate", c_void_p),
+        ("x_stride", c_int64), ("branch_stride", c_int64), ("gate_stride", c_int64),
+        ("scale", c_void_p), ("post_weight", c_void_p), ("post_bias", c_void_p), ("pre_weight", c_void_p), ("pre_bias", c_void_p),
+        ("y", c_void_p), ("h", c_void_p), ("stats", c_void_p),
+        ("x_codes", c_void_p), ("x_exps", c_void_p), ("branch_codes", c_void_p), ("branch_exps", c_void_p), ("gate_codes", c_void_p), ("gate_exps", c_void_p),
+        ("dy", c_void_p), ("dh", c_void_p), ("dy_stride", c_int64), ("dh_stride", c_int64),
+        ("dx", c_void_p), ("dbranch", c_void_p), ("dgate", c_void_p),
+        ("dscale", c_void_p), ("dpost_weight", c_void_p), ("dpost_bias", c_void_p), ("dpre_weight", c_void_p), ("dpre_bias", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
 
@@ -186,6 +204,25 @@ _SIGNATURES = {
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
+# include/schemanet_blocks.h, the second part of the C ABI
+BLOCKS_ABI_VERSION = 1
+_BLOCK_SIGNATURES = {
+    "sn_blocks_abi_version": (c_int, []),
+    "sn_checkpoint8": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_void_p, c_void_p]),
+    "sn_checkpoint8_restore": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p]),
+    "sn_checkpoint8_weight_grad_workspace": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "sn_checkpoint8_weight_grad": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                                           c_size_t, c_void_p]),
+    "sn_block_norms_forward": (c_int, [POINTER(BlockNormsArgs), c_void_p]),
+    "sn_block_norms_workspace": (c_size_t, [c_int64, c_int]),
+    "sn_block_norms_backward": (c_int, [POINTER(BlockNormsArgs), c_void_p]),
+    "sn_label_log_probs_workspace": (c_size_t, [c_int64, c_int64, c_int]),
+    "sn_label_log_probs": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_size_t, c_void_p]),
+    "sn_label_log_probs_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+}
+BLOCK_SYMBOLS = tuple(_BLOCK_SIGNATURES)
+
 
 def build(force=False):
     """hipcc-compile the library in-tree (cross-compiles for gfx950 without a GPU)."""
@@ -204,12 +241,14 @@ def load():
             f"schemanet HIP extension not built: {LIB_PATH} is missing (run `python -c 'import "
             f"__graft_entry__ as g; g.build()'` or `make -C schemanet-pytorch_amd`); there is no CPU fallback")
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in _SIGNATURES.items():
+    for name, (res, args) in (*_SIGNATURES.items(), *_BLOCK_SIGNATURES.items()):
         fn = getattr(lib, name)          # AttributeError if the .so does not export a declared symbol
         fn.restype = res
         fn.argtypes = args
     if lib.sn_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libschemanet_hip.so ABI {lib.sn_abi_version()} != expected {ABI_VERSION}")
+    if lib.sn_blocks_abi_version() != BLOCKS_ABI_VERSION:
+        raise RuntimeError(f"libschemanet_hip.so blocks ABI {lib.sn_blocks_abi_version()} != expected {BLOCKS_ABI_VERSION}")
     _lib = lib
     return lib
 

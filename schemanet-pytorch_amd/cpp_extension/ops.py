@@ -1548,3 +1548,8 @@ def class_votes_(pred, votes):
     with torch.cuda.device(dev):
         N.check(lib.sn_class_votes(N.ptr(p), B, K, N.ptr(votes), N.stream_ptr(dev)), "sn_class_votes")
     return votes
+
+
+# ------------------------------------------------------------------------------- residual blocks, 8-bit checkpoints, answers
+from .block_ops import (Checkpoint8, LabelLogProbs, checkpoint8, checkpoint8_weight_grad, gated_residual_norms,  # noqa: E402,F401
+                        label_log_probs, linear_checkpoint8)

@@ -1,5 +1,6 @@
 // ABI housekeeping: version, thread-local error string, device probe.
 #include "sn_common.h"
+#include "schemanet_blocks.h"
 
 #include <string.h>
 
@@ -17,6 +18,7 @@ void sn_set_error(const char *fmt, ...)
 }
 
 extern "C" int sn_abi_version(void) { return 12; }
+extern "C" int sn_blocks_abi_version(void) { return 1; }
 
 extern "C" const char *sn_last_error(void) { return g_err; }
 
