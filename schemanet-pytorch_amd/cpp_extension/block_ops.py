@@ -39,6 +39,35 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _launch(fn, what, dev, *args):
+    """fn(*args, current stream of dev) with dev as the current device.  The host's part of a small call is most of it (about 25 us a
+    forward call, and the autograd thread runs Python at a third of that speed): the device is only switched where it is another
+    one, and the stream is asked for as a number."""
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = fn(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc != 0:
+        N.check(rc, what)
+
+
+def _library():
+    return N._lib if N._lib is not None else N.require_gpu()
+
+
+def _once(backward):
+    """a backward pass without second derivatives: the wrapper that says so on their use is only taken under create_graph"""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return staticmethod(run)
+
+
 def _rows(t, width):
     """[..., width] as (tensor that holds the rows, stride of a row): a view where the rows lie evenly apart, a copy otherwise"""
     if t.stride(-1) != 1 and width > 1:
@@ -88,10 +117,8 @@ class Checkpoint8:
         _need(dtype in _TYPES, "checkpoint8: cannot restore to {}", dtype)
         out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
         if out.numel():
-            lib = N.require_gpu()
-            with torch.cuda.device(out.device):
-                N.check(lib.sn_checkpoint8_restore(_p(self.codes), _p(self.exps), self.codes.shape[0], self.shape[-1], _p(out), _TYPES[dtype],
-                                                   N.stream_ptr(out.device)), "sn_checkpoint8_restore")
+            _launch(_library().sn_checkpoint8_restore, "sn_checkpoint8_restore", out.device, _p(self.codes), _p(self.exps), self.codes.shape[0],
+                    self.shape[-1], _p(out), _TYPES[dtype])
         return out
 
 
@@ -113,11 +140,9 @@ def checkpoint8(x):
     x = x.detach()
     kept = _empty_checkpoint(x.shape, x.dtype, dev)
     if x.numel():
-        lib = N.require_gpu()
         v, stride = _rows(x, x.shape[-1])
-        with torch.cuda.device(dev):
-            N.check(lib.sn_checkpoint8(_p(v), _TYPES[x.dtype], kept.codes.shape[0], x.shape[-1], stride, _p(kept.codes), _p(kept.exps),
-                                       N.stream_ptr(dev)), "sn_checkpoint8")
+        _launch(_library().sn_checkpoint8, "sn_checkpoint8", dev, _p(v), _TYPES[x.dtype], kept.codes.shape[0], x.shape[-1], stride, _p(kept.codes),
+                _p(kept.exps))
     return kept
 
 
@@ -139,15 +164,14 @@ def checkpoint8_weight_grad(dy, kept, bias=True, out_dtype=None):
     out_f, in_f, rows = dy.shape[-1], kept.shape[-1], kept.codes.shape[0]
     if rows == 0:
         return (torch.zeros((out_f, in_f), dtype=out_dtype, device=dev), torch.zeros(out_f, dtype=out_dtype, device=dev) if bias else None)
-    lib = N.require_gpu()
+    lib = _library()
     dw = torch.empty((out_f, in_f), dtype=out_dtype, device=dev)
     db = torch.empty(out_f, dtype=out_dtype, device=dev) if bias else None
     v, stride = _rows(dy, out_f)
     size = lib.sn_checkpoint8_weight_grad_workspace(rows, out_f, in_f, _TYPES[dy.dtype])
     ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        N.check(lib.sn_checkpoint8_weight_grad(_p(v), _TYPES[dy.dtype], stride, _p(kept.codes), _p(kept.exps), rows, out_f, in_f, _p(dw), _p(db),
-                                               _TYPES[out_dtype], _p(ws), size, N.stream_ptr(dev)), "sn_checkpoint8_weight_grad")
+    _launch(lib.sn_checkpoint8_weight_grad, "sn_checkpoint8_weight_grad", dev, _p(v), _TYPES[dy.dtype], stride, _p(kept.codes), _p(kept.exps), rows, out_f,
+            in_f, _p(dw), _p(db), _TYPES[out_dtype], _p(ws), size)
     return dw, db
 
 
@@ -169,8 +193,7 @@ class _LinearCheckpoint8(torch.autograd.Function):
         ctx.shape, ctx.scale, ctx.has_bias = tuple(x.shape), wp.scale, bias is not None
         return y[0] if x.dim() == 2 else y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         from . import ops
         weight = ctx.saved_tensors[0]
@@ -218,7 +241,7 @@ def _norm_args(x, branch, gate, scale, post, pre, rms, eps, n_valid):
 
 
 def _norms_forward(x, branch, gate, scale, post, pre, rms, eps, n_valid, train, keep8):
-    lib = N.require_gpu()
+    lib = _library()
     dev, width = x.device, x.shape[-1]
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     h = torch.empty(x.shape, dtype=x.dtype, device=dev) if pre[0] is not None else None
@@ -242,8 +265,7 @@ def _norms_forward(x, branch, gate, scale, post, pre, rms, eps, n_valid, train, 
             a.branch_codes, a.branch_exps = _p(kept[1].codes), _p(kept[1].exps)
             if gate is not None:
                 a.gate_codes, a.gate_exps = _p(kept[2].codes), _p(kept[2].exps)
-    with torch.cuda.device(dev):
-        N.check(lib.sn_block_norms_forward(byref(a), N.stream_ptr(dev)), "sn_block_norms_forward")
+    _launch(lib.sn_block_norms_forward, "sn_block_norms_forward", dev, byref(a))
     return y, h, stats, kept
 
 
@@ -261,8 +283,7 @@ class _GatedResidualNorms(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return y if h is None else (y, h)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dh=None):
         scale, post_w, post_b, pre_w, pre_b, n_valid, stats, *held = ctx.saved_tensors
         shape, dtype, rms, eps = ctx.opts
@@ -272,7 +293,7 @@ class _GatedResidualNorms(torch.autograd.Function):
         if stats is None:                                                   # no rows
             whole = [torch.zeros(shape, dtype=dtype, device=dev) if want[i] else None for i in range(3)]
             return (*whole, *(torch.zeros_like(p) if p is not None and want[3 + i] else None for i, p in enumerate(params)), None, None, None, None)
-        lib = N.require_gpu()
+        lib = _library()
         x_like = torch.empty(shape, dtype=dtype, device=dev)                # dx, or only the sizes
         a = _norm_args(x_like, None, None, scale, (post_w, post_b), (pre_w, pre_b), rms, eps, n_valid)
         a.stats = _p(stats)
@@ -310,8 +331,7 @@ class _GatedResidualNorms(torch.autograd.Function):
         size = lib.sn_block_norms_workspace(a.rows, width)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = _p(ws), size
-        with torch.cuda.device(dev):
-            N.check(lib.sn_block_norms_backward(byref(a), N.stream_ptr(dev)), "sn_block_norms_backward")
+        _launch(lib.sn_block_norms_backward, "sn_block_norms_backward", dev, byref(a))
         return (dx, dbranch, dgate, *grads, None, None, None, None)
 
 
@@ -368,7 +388,7 @@ LabelLogProbs = namedtuple("LabelLogProbs", ["log_probs", "entropy", "top_log_pr
 
 
 def _scores_forward(logits, target, ignore_index, topk):
-    lib = N.require_gpu()
+    lib = _library()
     dev, n = logits.device, logits.shape[-1]
     lead = target.shape
     rows = target.numel()
@@ -381,9 +401,8 @@ def _scores_forward(logits, target, ignore_index, topk):
         v, stride = _rows(logits, n)
         size = lib.sn_label_log_probs_workspace(rows, n, topk)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            N.check(lib.sn_label_log_probs(_p(v), _TYPES[logits.dtype], rows, n, stride, _p(target), ignore_index, topk, _p(lp), _p(ent), _p(stats),
-                                           _p(top_lp), _p(top_ids), _p(ws), size, N.stream_ptr(dev)), "sn_label_log_probs")
+        _launch(lib.sn_label_log_probs, "sn_label_log_probs", dev, _p(v), _TYPES[logits.dtype], rows, n, stride, _p(target), ignore_index, topk, _p(lp), _p(ent),
+                _p(stats), _p(top_lp), _p(top_ids), _p(ws), size)
     return lp, ent, stats, top_lp, top_ids
 
 
@@ -400,22 +419,20 @@ class _LabelLogProbs(torch.autograd.Function):
         ctx.mark_non_differentiable(top_lp, top_ids)
         return lp, ent, top_lp, top_ids
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g_lp, g_ent, *unused):
         logits, target, stats = ctx.saved_tensors
         if g_lp is None and g_ent is None:
             return None, None, None, None
-        lib = N.require_gpu()
+        lib = _library()
         dev, n, rows = logits.device, logits.shape[-1], target.numel()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         if rows:
             g_lp = None if g_lp is None else g_lp.float().contiguous()
             g_ent = None if g_ent is None else g_ent.float().contiguous()
             v, stride = _rows(logits, n)
-            with torch.cuda.device(dev):
-                N.check(lib.sn_label_log_probs_backward(_p(v), _TYPES[logits.dtype], rows, n, stride, _p(target), ctx.ignore_index, _p(stats), _p(g_lp),
-                                                        _p(g_ent), _p(grad), N.stream_ptr(dev)), "sn_label_log_probs_backward")
+            _launch(lib.sn_label_log_probs_backward, "sn_label_log_probs_backward", dev, _p(v), _TYPES[logits.dtype], rows, n, stride, _p(target),
+                    ctx.ignore_index, _p(stats), _p(g_lp), _p(g_ent), _p(grad))
         return grad, None, None, None
 
 
