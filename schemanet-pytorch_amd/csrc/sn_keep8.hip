@@ -55,199 +55,356 @@ __global__ __launch_bounds__(kPackThreads) void restore8_kernel(const uint8_t *c
 }
 
 // ------------------------------------------------------------------------------------------
-// dW: tiles of 128 x 128 outputs, 64 rows a step, four waves of 64 x 64 (2 x 2 MFMA 32x32x16).  Both operands lie with the
-// summed index outermost, so a thread takes 8 rows of 4 columns, turns them in registers (the bf16 conversion pairs two ROWS
-// into a word) and writes 8 consecutive k of one column to LDS as the matrix instruction wants them.
-constexpr int kTile = 128, kStepRows = 64, kGradThreads = 256;
-constexpr int kPlane = kTile * kStepRows;                   // bf16 elements of one operand piece in LDS (16 KiB)
-
-// 16-byte chunk c (8 k) of column m: the eight chunks of a column are rotated so that both the writes (columns 4 apart) and the
-// reads (neighbouring columns) of eight lanes fall on different banks
-__device__ __forceinline__ int lds_at(int m, int c) { return m * kStepRows + ((c ^ ((m ^ (m >> 3)) & 7)) << 3); }
+// dW: a workgroup owns TILE x TILE outputs of one split of the summed rows, BK rows a step, MFMA 32x32x16 on wave tiles of
+// 128 x 64 (TILE 256, eight waves) or 64 x 64 (TILE 128, four).  Both operands lie with the summed index outermost, so a
+// staging thread takes 8 rows of UC columns, turns them in registers (the bf16 conversion pairs two ROWS into a word) and
+// writes 8 consecutive rows of one column to LDS, as the matrix instruction wants them.  Half of the waves stage dY, the other
+// half the kept codes; two LDS buffers, one barrier a step; the dY waves stage before their products and the code waves after
+// them, so that on every SIMD the vector work of one wave runs under the matrix instructions of the other.
+typedef uint32_t u32;
 
 template <int DT> constexpr int pieces() { return DT == SN_F32 ? 3 : DT == SN_F16 ? 2 : 1; }
 
-template <int DT>
-__global__ __launch_bounds__(kGradThreads) void weight_grad8_kernel(const void *dy, int64_t dy_stride, const uint8_t *codes, const uint8_t *exps, int64_t rows,
-                                                                    int out_f, int in_f, int rows_per_split, void *dw, void *db, int out_dtype, float *part_w,
-                                                                    float *part_b)
+template <int DT, int TILE> struct Grad {
+    static constexpr int P = pieces<DT>();
+    static constexpr int BK = P == 1 ? 64 : 32;              // rows of a step: two buffers of P + 1 pieces in 128 KiB
+    static constexpr int UC = P == 1 ? 8 : 4;                // columns of a staging thread
+    static constexpr int kWaves = TILE == 256 ? 8 : 4, kThreads = kWaves * 64;
+    static constexpr int kPlane = TILE * BK;                 // bf16 elements of one piece
+    static constexpr int kBuffer = (P + 1) * kPlane;
+    static constexpr int kGroups = TILE / UC;                // column groups
+    static constexpr int MT = TILE == 256 ? 4 : 2, NT = 2;   // 32 x 32 products of a wave
+    static constexpr int kBlocks = TILE / 32;                // checkpoint blocks of a row of the tile
+    static constexpr int kKg = 64 / kGroups > 0 ? 64 / kGroups : 1;      // row groups of a staging wave
+    static constexpr int JR = 64 / (kKg * kBlocks);          // rows of a group whose exponents one register of the wave holds
+    static_assert(kGroups * (BK / 8) * 2 == kThreads, "half of the threads stage each operand");
+    static_assert(JR == 4 || JR == 8, "a wave's exponents in one or two registers");
+};
+
+// 16-byte chunk c (8 rows) of column m.  The chunks of a column are rotated so that the writes (columns UC apart) and the reads
+// (neighbouring columns) of eight lanes fall on different banks (BK 32: the writes on half of them)
+template <int BK> __device__ __forceinline__ int lds_at(int m, int c)
 {
-    constexpr int P = pieces<DT>();
-    extern __shared__ uint16_t lds[];                        // P pieces of dY, then kept
-    uint16_t *const lb = lds + P * kPlane;
-    const int tiles_i = (in_f + kTile - 1) / kTile;
-    const int o0 = (blockIdx.x / tiles_i) * kTile, i0 = (blockIdx.x % tiles_i) * kTile;
-    const int64_t r_begin = (int64_t)blockIdx.y * rows_per_split;
+    if constexpr (BK == 64) return m * BK + ((c ^ ((m ^ (m >> 3)) & 7)) << 3);
+    else return m * BK + ((c ^ (((m >> 1) ^ (m >> 3)) & 3)) << 3);
+}
+
+template <int DT, int NW> __device__ __forceinline__ float element(const u32 (&w)[NW], int j)
+{
+    if constexpr (DT == SN_F32) return __uint_as_float(w[j]);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j / 2] >> (16 * (j & 1))));
+}
+
+// SMALL: sizes under one tile or one step, rows too far apart for 32-bit offsets - every load is tested.  Otherwise none is: the last
+// tile of a row or column of tiles and the last step of a split are moved back to where they are whole; outputs that two tiles
+// share come out of both with the same bits, rows that a split has had already are cleared from dY before they are staged.
+template <int DT, int TILE, bool SMALL>
+__global__ __launch_bounds__((Grad<DT, TILE>::kThreads), 2) void weight_grad8_kernel(const void *dy, int64_t dy_stride, const uint8_t *codes, const uint8_t *exps,
+                                                                                 int64_t rows, int out_f, int in_f, int splits, int rows_per_split, void *dw,
+                                                                                 void *db, int out_dtype, float *part_w, float *part_b)
+{
+    using G = Grad<DT, TILE>;
+    constexpr int P = G::P, BK = G::BK, UC = G::UC, SIZE = DT == SN_F32 ? 4 : 2;
+    extern __shared__ uint16_t lds[];
+    // the workgroups of one XCD (every eighth) take neighbouring tiles of the same rows: they share panels in its L2
+    const int tiles_i = (in_f + TILE - 1) / TILE, tiles = tiles_i * ((out_f + TILE - 1) / TILE), total = tiles * splits;
+    const int xcd = blockIdx.x & 7, each = total >> 3, rest = total & 7;
+    const int work = xcd * each + (xcd < rest ? xcd : rest) + (int)(blockIdx.x >> 3);
+    const int split = work / tiles, tile = work - split * tiles;
+    const int npad = (in_f + 31) & ~31, nblk = npad >> 5;
+    int o0 = (tile / tiles_i) * TILE, i0 = (tile % tiles_i) * TILE;
+    if constexpr (!SMALL) {
+        o0 = o0 + TILE <= out_f ? o0 : out_f - TILE;
+        i0 = i0 + TILE <= npad ? i0 : npad - TILE;
+    }
+    const int64_t r_begin = (int64_t)split * rows_per_split;
     const int64_t r_end = r_begin + rows_per_split < rows ? r_begin + rows_per_split : rows;
-    const int npad = (in_f + 31) & ~31;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int cg = t & 31, kg = t >> 5;                      // columns 4 cg .. + 3, rows 8 kg .. + 7 of a step
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    const bool role_x = wave >= G::kWaves / 2;               // stages the kept codes
+    const int unit = role_x ? t - G::kThreads / 2 : t;
+    const int cg = unit % G::kGroups, kg = unit / G::kGroups;
+    const int wm = TILE == 256 ? (wave & 1) * 128 : (wave & 1) * 64, wn = (wave >> 1) * 64;
     const bool sums = db && i0 == 0;
 
-    f32x16 acc[2][2] = {};
-    float bias[4] = {};
-    uint32_t ra[8][words<DT, 4>()], rq[8], re[8];
+    f32x16 acc[G::MT][G::NT] = {};
+    float bias[UC] = {};
+    u32 raw[8][UC * SIZE / 4];                               // dY, or (the first words) codes
+    u32 ex[8 / G::JR];
 
+    // exponents: one or two loads for the wave's rows and blocks, handed round by lane
+    const int ex_b = i0 / 32 + lane % G::kBlocks;
+    const int ex_row = (kg - lane / G::kGroups + lane / (G::kBlocks * G::JR)) * 8 + (lane / G::kBlocks) % G::JR;
+    // a scalar row address and a 32-bit offset of the lane
+    const u32 lane_off = role_x ? (u32)(kg * 8 * npad + UC * cg) : (u32)(kg * 8 * (int)dy_stride + UC * cg) * SIZE;
+    const u32 ex_off = (u32)(ex_row * nblk + ex_b);
     auto fetch = [&](int64_t r0) {
+        if constexpr (!SMALL) {
+            r0 = r0 + BK <= r_end ? r0 : r_end - BK;
+            if (!role_x) {
+                const char *const base = (const char *)dy + (r0 * dy_stride + o0) * SIZE;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int64_t r = r0 + kg * 8 + k;
-            const bool in = r < r_end;
-            load_raw<DT, 4>(ra[k], (const char *)dy + (in ? r : r_begin) * dy_stride * (DT == SN_F32 ? 4 : 2), o0 + 4 * cg, in ? out_f : 0);
-            rq[k] = 0u;
-            re[k] = 8u;
-            if (in && i0 + 4 * cg < npad) {
-                rq[k] = *reinterpret_cast<const uint32_t *>(codes + r * npad + i0 + 4 * cg);
-                re[k] = exps[r * (npad / 32) + (i0 + 4 * cg) / 32];
+                for (int k = 0; k < 8; ++k) load_words<UC * SIZE / 4>(raw[k], base + k * dy_stride * SIZE + lane_off);
+            } else {
+                const uint8_t *const base = codes + r0 * npad + i0, *const ebase = exps + r0 * nblk;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const u32 *src = (const u32 *)(base + k * npad + lane_off);
+#pragma unroll
+                    for (int q = 0; q < UC / 4; ++q) raw[k][q] = src[q];
+                }
+#pragma unroll
+                for (int q = 0; q < 8 / G::JR; ++q) ex[q] = (ebase + q * G::JR * nblk)[ex_off];
+            }
+        } else if (!role_x) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int64_t r = r0 + kg * 8 + k;
+                const bool in = r < r_end;
+                load_raw<DT, UC>(raw[k], (const char *)dy + (in ? r : r_begin) * dy_stride * SIZE, o0 + UC * cg, in ? out_f : 0);
+            }
+        } else {
+            const int j = i0 + UC * cg;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int64_t r = r0 + kg * 8 + k;
+                const bool in = r < r_end && j < npad;
+                const u32 *src = (const u32 *)(codes + (in ? r * npad + j : 0));
+#pragma unroll
+                for (int q = 0; q < UC / 4; ++q) raw[k][q] = in ? src[q] : 0u;
+            }
+#pragma unroll
+            for (int q = 0; q < 8 / G::JR; ++q) {
+                const int64_t r = r0 + ex_row + q * G::JR;
+                ex[q] = r < r_end && ex_b < nblk ? exps[r * nblk + ex_b] : 8u;
             }
         }
     };
-    auto stage = [&]() {
-        float v[8][4];
+    auto stage = [&](uint16_t *buf, int64_t r0) {
+        if (!role_x) {
+            if (!SMALL && r0 + BK > r_end) {                 // (the rows before r0 of a step that was moved back)
+                const int had = (int)(r0 + BK - r_end) - kg * 8;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) unpack<DT, 4>(v[k], ra[k]);
-        if (sums) {
+                for (int k = 0; k < 8; ++k)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+                    for (int q = 0; q < UC * SIZE / 4; ++q) raw[k][q] = k < had ? 0u : raw[k][q];
+            }
+            if (sums) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) bias[j] += v[k][j];
-        }
+                for (int k = 0; k < 8; ++k) {
+                    float v[UC];
+                    unpack<DT, UC>(v, raw[k]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int at = lds_at(4 * cg + j, kg);
-            uint32_t w[P][4];
+                    for (int j = 0; j < UC; ++j) bias[j] += v[j];
+                }
+            }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float a = v[2 * k][j], b = v[2 * k + 1][j];
+            for (int j = 0; j < UC; ++j) {
+                const int at = lds_at<BK>(UC * cg + j, kg);
+                u32 w[P][4];
 #pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    w[p][k] = pack_bf16(a, b);
-                    if (p + 1 < P) {                         // what the piece leaves is exact in fp32
-                        a -= __uint_as_float(w[p][k] << 16);
-                        b -= __uint_as_float(w[p][k] & 0xFFFF0000u);
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (DT == SN_BF16) {           // already bf16: two rows' halves into a word
+                        w[0][k] = (j & 1) ? __builtin_amdgcn_perm(raw[2 * k + 1][j / 2], raw[2 * k][j / 2], 0x07060302u)
+                                          : __builtin_amdgcn_perm(raw[2 * k + 1][j / 2], raw[2 * k][j / 2], 0x05040100u);
+                    } else {
+                        float a = element<DT>(raw[2 * k], j), b = element<DT>(raw[2 * k + 1], j);
+#pragma unroll
+                        for (int p = 0; p < P; ++p) {
+                            w[p][k] = pack_bf16(a, b);
+                            if (p + 1 < P) {                 // what the piece leaves is exact in fp32
+                                a -= __uint_as_float(w[p][k] << 16);
+                                b -= __uint_as_float(w[p][k] & 0xFFFF0000u);
+                            }
+                        }
                     }
                 }
+#pragma unroll
+                for (int p = 0; p < P; ++p) *reinterpret_cast<uint4 *>(buf + p * G::kPlane + at) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+            }
+        } else {
+            uint16_t *const bx = buf + P * G::kPlane;
+            const int from = ((lane / G::kGroups) * G::JR) * G::kBlocks + (cg * UC) / 32;
+            float step[8];
+#pragma unroll
+            for (int q = 0; q < 8 / G::JR; ++q) {
+                const int held = __float_as_int(block_step(ex[q]));
+#pragma unroll
+                for (int k = 0; k < G::JR; ++k) step[q * G::JR + k] = __int_as_float(__builtin_amdgcn_ds_bpermute((from + k * G::kBlocks) * 4, held));
             }
 #pragma unroll
-            for (int p = 0; p < P; ++p) *reinterpret_cast<uint4 *>(lds + p * kPlane + at) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
-        }
+            for (int j = 0; j < UC; ++j) {
+                u32 w[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t q[1] = {rq[k]};
-            decode<4>(v[k], q, re[k]);
+                for (int k = 0; k < 4; ++k)
+                    w[k] = pack_bf16((float)(int8_t)(raw[2 * k][j / 4] >> (8 * (j & 3))) * step[2 * k],
+                                     (float)(int8_t)(raw[2 * k + 1][j / 4] >> (8 * (j & 3))) * step[2 * k + 1]);
+                *reinterpret_cast<uint4 *>(bx + lds_at<BK>(UC * cg + j, kg)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
+    };
+    // operands of one group of 16 rows are read while the previous group multiplies (P = 1; more pieces: their products are long enough)
+    constexpr int KK = BK / 16, AHEAD = P == 1 ? 2 : 1;
+    auto multiply = [&](const uint16_t *buf) {
+        const uint16_t *const bx = buf + P * G::kPlane;
+        bf16x8 a[AHEAD][G::MT][P], b[AHEAD][G::NT];
+        auto read = [&](int kk, int s) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint4 w;
-            w.x = pack_bf16(v[0][j], v[1][j]); w.y = pack_bf16(v[2][j], v[3][j]);
-            w.z = pack_bf16(v[4][j], v[5][j]); w.w = pack_bf16(v[6][j], v[7][j]);
-            *reinterpret_cast<uint4 *>(lb + lds_at(4 * cg + j, kg)) = w;
+            for (int n = 0; n < G::NT; ++n) b[s][n] = *reinterpret_cast<const bf16x8 *>(bx + lds_at<BK>(wn + n * 32 + (lane & 31), 2 * kk + (lane >> 5)));
+#pragma unroll
+            for (int m = 0; m < G::MT; ++m)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                    a[s][m][p] = *reinterpret_cast<const bf16x8 *>(buf + p * G::kPlane + lds_at<BK>(wm + m * 32 + (lane & 31), 2 * kk + (lane >> 5)));
+        };
+        if constexpr (AHEAD == 2) read(0, 0);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int s = kk % AHEAD;
+            if constexpr (AHEAD == 1) read(kk, 0);
+            else if (kk + 1 < KK) read(kk + 1, (kk + 1) % AHEAD);
+#pragma unroll
+            for (int m = 0; m < G::MT; ++m)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int n = 0; n < G::NT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[s][m][p], b[s][n], acc[m][n], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);               // (or the compiler reads all groups at once and spills)
         }
     };
 
-    if (r_begin < r_end) fetch(r_begin);
-    for (int64_t r0 = r_begin; r0 < r_end; r0 += kStepRows) {
-        stage();
-        __syncthreads();
-        if (r0 + kStepRows < r_end) fetch(r0 + kStepRows);
-#pragma unroll
-        for (int kk = 0; kk < kStepRows / 16; ++kk) {
-            bf16x8 b[2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) b[n] = *reinterpret_cast<const bf16x8 *>(lb + lds_at(wn + n * 32 + (lane & 31), 2 * kk + (lane >> 5)));
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const bf16x8 a = *reinterpret_cast<const bf16x8 *>(lds + p * kPlane + lds_at(wm + m * 32 + (lane & 31), 2 * kk + (lane >> 5)));
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[n], acc[m][n], 0, 0, 0);
-                }
+    // (every split has rows: rows_per_split and splits come from split_rows)
+    fetch(r_begin);
+    stage(lds, r_begin);
+    if (r_begin + BK < r_end) fetch(r_begin + BK);
+    __syncthreads();
+    int cur = 0;
+    for (int64_t r0 = r_begin; r0 < r_end; r0 += BK, cur ^= 1) {
+        uint16_t *const here = lds + cur * G::kBuffer, *const next = lds + (cur ^ 1) * G::kBuffer;
+        const bool more = r0 + BK < r_end, after = r0 + 2 * BK < r_end;
+        if (!role_x) {
+            if (more) stage(next, r0 + BK);
+            if (after) fetch(r0 + 2 * BK);
+            multiply(here);
+        } else {
+            multiply(here);
+            if (more) stage(next, r0 + BK);
+            if (after) fetch(r0 + 2 * BK);
         }
         __syncthreads();
     }
 
     // C of the 32x32 instruction: column lane & 31, row (i & 3) + 8 (i >> 2) + 4 (lane >> 5)
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < G::MT; ++m)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < G::NT; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int o = o0 + wm + m * 32 + (i & 3) + 8 * (i >> 2) + 4 * (lane >> 5), c = i0 + wn + n * 32 + (lane & 31);
                 if (o < out_f && c < in_f) {
-                    if (part_w) part_w[((int64_t)blockIdx.y * out_f + o) * in_f + c] = acc[m][n][i];
+                    if (part_w) part_w[((int64_t)split * out_f + o) * in_f + c] = acc[m][n][i];
                     else store_any(dw, out_dtype, (int64_t)o * in_f + c, acc[m][n][i]);
                 }
             }
-    if (sums) {
-        float *red = reinterpret_cast<float *>(lds);         // [8 row groups][128 columns]
+    if (sums) {                                              // (the last turn ended with a barrier: LDS is free)
+        float *red = reinterpret_cast<float *>(lds);         // [BK / 8 row groups][TILE columns]
+        if (!role_x) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) red[kg * kTile + 4 * cg + j] = bias[j];
+            for (int j = 0; j < UC; ++j) red[kg * TILE + UC * cg + j] = bias[j];
+        }
         __syncthreads();
-        if (t < kTile && o0 + t < out_f) {
+        if (t < TILE && o0 + t < out_f) {
             float s = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s += red[k * kTile + t];
-            if (part_b) part_b[(int64_t)blockIdx.y * out_f + o0 + t] = s;
+            for (int k = 0; k < BK / 8; ++k) s += red[k * TILE + t];
+            if (part_b) part_b[(int64_t)split * out_f + o0 + t] = s;
             else store_any(db, out_dtype, o0 + t, s);
         }
     }
 }
 
-// the splits' partial results, added in order: 4 elements a thread; the last blocks take db
+// the splits' partial results: 4 cells a thread, the splits dealt to four groups of threads, added in a fixed order.  The cells of
+// dW and db lie behind one another (part_b = part_w + splits * cells of dW); a thread's four never span both.
 __global__ __launch_bounds__(256) void weight_grad8_join_kernel(const float *part_w, const float *part_b, int splits, int64_t cells, int out_f, void *dw, void *db,
                                                                 int out_dtype)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < cells) {
-        float s = 0.0f;
-#pragma unroll 8
-        for (int p = 0; p < splits; ++p) s += part_w[(int64_t)p * cells + i];
-        store_any(dw, out_dtype, i, s);
-    } else if (db && i - cells < out_f) {
-        float s = 0.0f;
-        for (int p = 0; p < splits; ++p) s += part_b[(int64_t)p * out_f + (i - cells)];
-        store_any(db, out_dtype, i - cells, s);
+    __shared__ float4 red[4][64];
+    const int q = threadIdx.x & 63, group = threadIdx.x >> 6;
+    const int64_t quads = (cells + 3) / 4, i = (int64_t)blockIdx.x * 64 + q;
+    const bool bias = i >= quads;
+    const int64_t c = bias ? (i - quads) * 4 : i * 4, n = bias ? out_f : cells;
+    const float *src = bias ? part_b : part_w;
+    float s[4] = {};
+    if (c < n && (!bias || db)) {
+#pragma unroll 4
+        for (int p = group; p < splits; p += 4) {
+            u32 w[4];
+            load_raw<SN_F32, 4>(w, src + p * n + c, 0, n - c < 4 ? (int)(n - c) : 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] += __uint_as_float(w[k]);
+        }
+    }
+    red[group][q] = make_float4(s[0], s[1], s[2], s[3]);
+    __syncthreads();
+    if (group == 0 && c < n && (!bias || db)) {
+        const float4 a = red[1][q], b = red[2][q], d = red[3][q];
+        const float v[4] = {(s[0] + a.x) + (b.x + d.x), (s[1] + a.y) + (b.y + d.y), (s[2] + a.z) + (b.z + d.z), (s[3] + a.w) + (b.w + d.w)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (c + k < n) store_any(bias ? db : dw, out_dtype, c + k, v[k]);
     }
 }
 
-// splits of the summed rows: enough workgroups for two on each of the 256 compute units, at least 256 rows a split
-struct Split { int n, rows; };
-Split split_rows(int64_t rows, int out_f, int in_f)
+int64_t tiles_of(int out_f, int in_f, int tile) { return (int64_t)((out_f + tile - 1) / tile) * ((in_f + tile - 1) / tile); }
+
+// Tile and splits of the summed rows: the large tile where its own number (with up to four splits) fills the 256 compute units,
+// the small one otherwise; then enough splits for two small or one large workgroup on each compute unit, at least 256 rows a split
+struct Split { int tile, n, rows; bool small; };
+Split split_rows(int64_t rows, int out_f, int in_f, int64_t dy_stride)
 {
-    const int64_t tiles = (int64_t)((out_f + kTile - 1) / kTile) * ((in_f + kTile - 1) / kTile);
-    int64_t n = 512 / tiles;
+    Split s;
+    const int npad = (in_f + 31) & ~31;
+    s.small = rows < 64 || out_f < 128 || npad < 128 || dy_stride >= (1 << 22) || npad >= (1 << 22);
+    s.tile = !s.small && out_f >= 256 && npad >= 256 && tiles_of(out_f, in_f, 256) >= 64 ? 256 : 128;
+    const int64_t tiles = tiles_of(out_f, in_f, s.tile);
+    int64_t n = (s.tile == 256 ? 256 : 512) / tiles;
     const int64_t most = (rows + 255) / 256;
-    n = n < 1 ? 1 : n;
     n = n > most ? most : n;
     n = n < 1 ? 1 : n;
     int64_t per = (rows + n - 1) / n;
-    per = (per + kStepRows - 1) / kStepRows * kStepRows;
-    per = per < kStepRows ? kStepRows : per;
-    n = rows ? (rows + per - 1) / per : 1;
-    return Split{(int)n, (int)per};
+    per = (per + 63) / 64 * 64;
+    s.rows = (int)(per < 64 ? 64 : per);
+    s.n = rows ? (int)((rows + s.rows - 1) / s.rows) : 1;
+    return s;
+}
+
+template <int DT, int TILE, bool SMALL>
+int launch_tile(const Split &sp, const void *dy, int64_t dy_stride, const void *codes, const void *exps, int64_t rows, int out_f, int in_f, void *dw, void *db,
+                int out_dtype, float *part_w, float *part_b, hipStream_t st)
+{
+    using G = Grad<DT, TILE>;
+    const size_t lds = (size_t)2 * G::kBuffer * 2;
+    const int rc = sn_ensure_dynamic_lds((const void *)weight_grad8_kernel<DT, TILE, SMALL>, lds, "sn_checkpoint8_weight_grad");
+    if (rc != SN_OK) return rc;
+    hipLaunchKernelGGL((weight_grad8_kernel<DT, TILE, SMALL>), dim3((unsigned)(tiles_of(out_f, in_f, TILE) * sp.n)), dim3(G::kThreads), lds, st, dy, dy_stride,
+                       (const uint8_t *)codes, (const uint8_t *)exps, rows, out_f, in_f, sp.n, sp.rows, dw, db, out_dtype, part_w, part_b);
+    SN_CHECK_LAUNCH("sn_checkpoint8_weight_grad");
+    return SN_OK;
 }
 
 template <int DT>
 int launch_grad(const void *dy, int64_t dy_stride, const void *codes, const void *exps, int64_t rows, int out_f, int in_f, void *dw, void *db, int out_dtype,
                 void *workspace, hipStream_t st)
 {
-    const Split sp = split_rows(rows, out_f, in_f);
-    const int64_t tiles = (int64_t)((out_f + kTile - 1) / kTile) * ((in_f + kTile - 1) / kTile), cells = (int64_t)out_f * in_f;
+    const Split sp = split_rows(rows, out_f, in_f, dy_stride);
+    const int64_t cells = (int64_t)out_f * in_f;
     float *part_w = sp.n > 1 ? (float *)workspace : nullptr, *part_b = sp.n > 1 ? part_w + sp.n * cells : nullptr;
-    const size_t lds = (size_t)(pieces<DT>() + 1) * kPlane * 2;
-    const int rc = sn_ensure_dynamic_lds((const void *)weight_grad8_kernel<DT>, lds, "sn_checkpoint8_weight_grad");
-    if (rc != SN_OK) return rc;
-    hipLaunchKernelGGL(weight_grad8_kernel<DT>, dim3((unsigned)tiles, sp.n), dim3(kGradThreads), lds, st, dy, dy_stride, (const uint8_t *)codes, (const uint8_t *)exps,
-                       rows, out_f, in_f, sp.rows, dw, db, out_dtype, part_w, part_b);
-    SN_CHECK_LAUNCH("sn_checkpoint8_weight_grad");
-    if (sp.n > 1) {
-        hipLaunchKernelGGL(weight_grad8_join_kernel, dim3((unsigned)((cells + (db ? out_f : 0) + 255) / 256)), dim3(256), 0, st, part_w, part_b, sp.n, cells, out_f,
-                           dw, db, out_dtype);
-        SN_CHECK_LAUNCH("sn_checkpoint8_weight_grad (join)");
-    }
+    const auto launch = sp.small ? launch_tile<DT, 128, true> : sp.tile == 256 ? launch_tile<DT, 256, false> : launch_tile<DT, 128, false>;
+    const int rc = launch(sp, dy, dy_stride, codes, exps, rows, out_f, in_f, dw, db, out_dtype, part_w, part_b, st);
+    if (rc != SN_OK || sp.n == 1) return rc;
+    const int64_t quads = (cells + 3) / 4 + (db ? (out_f + 3) / 4 : 0);
+    hipLaunchKernelGGL(weight_grad8_join_kernel, dim3((unsigned)((quads + 63) / 64)), dim3(256), 0, st, part_w, part_b, sp.n, cells, out_f, dw, db, out_dtype);
+    SN_CHECK_LAUNCH("sn_checkpoint8_weight_grad (join)");
     return SN_OK;
 }
 
@@ -292,8 +449,10 @@ extern "C" int sn_checkpoint8_restore(const void *codes, const void *exps, int64
 extern "C" size_t sn_checkpoint8_weight_grad_workspace(int64_t rows, int out_features, int in_features, int dy_dtype)
 {
     if (rows < 0 || out_features < 1 || in_features < 1 || dy_dtype < 0 || dy_dtype > 2) return 0;
-    const Split sp = split_rows(rows, out_features, in_features);
-    return sp.n > 1 ? (size_t)sp.n * ((size_t)out_features * in_features + out_features) * sizeof(float) : 16;
+    // (the stride of dy decides between two splits: room for either)
+    const int n = split_rows(rows, out_features, in_features, out_features).n, far = split_rows(rows, out_features, in_features, 1 << 22).n;
+    const int most = n > far ? n : far;
+    return most > 1 ? (size_t)most * ((size_t)out_features * in_features + out_features) * sizeof(float) : 16;
 }
 
 extern "C" int sn_checkpoint8_weight_grad(const void *dy, int dy_dtype, int64_t dy_row_stride, const void *codes, const void *exps, int64_t rows, int out_features,
