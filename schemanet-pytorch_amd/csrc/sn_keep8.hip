@@ -357,15 +357,18 @@ __global__ __launch_bounds__(256) void weight_grad8_join_kernel(const float *par
 
 int64_t tiles_of(int out_f, int in_f, int tile) { return (int64_t)((out_f + tile - 1) / tile) * ((in_f + tile - 1) / tile); }
 
-// Tile and splits of the summed rows: the large tile where its own number (with up to four splits) fills the 256 compute units,
-// the small one otherwise; then enough splits for two small or one large workgroup on each compute unit, at least 256 rows a split
+// Tile and splits of the summed rows.  The large tile where at least 4 of them, times splits, give each of the 256 compute units one
+// with 512 rows or more (32768 rows, bf16: 1024 x 1024 131 us on small tiles, 98 on large ones; 512 x 512 42.0, 41.6; 8192 rows of 512 x 1024
+// 32.0, 37.4), the small one otherwise; then enough splits for two small or one large workgroup on each compute unit (fewer leave
+// units idle, more write partial sums: 1024 x 1024, 512 workgroups of the large tile 117 us, 128 of them 140), at least 256 rows a split
 struct Split { int tile, n, rows; bool small; };
 Split split_rows(int64_t rows, int out_f, int in_f, int64_t dy_stride)
 {
     Split s;
     const int npad = (in_f + 31) & ~31;
     s.small = rows < 64 || out_f < 128 || npad < 128 || dy_stride >= (1 << 22) || npad >= (1 << 22);
-    s.tile = !s.small && out_f >= 256 && npad >= 256 && tiles_of(out_f, in_f, 256) >= 64 ? 256 : 128;
+    const int64_t large = tiles_of(out_f, in_f, 256);
+    s.tile = !s.small && out_f >= 256 && npad >= 256 && large >= 4 && rows * large >= 256 * 512 ? 256 : 128;
     const int64_t tiles = tiles_of(out_f, in_f, s.tile);
     int64_t n = (s.tile == 256 ? 256 : 512) / tiles;
     const int64_t most = (rows + 255) / 256;
