@@ -17,13 +17,13 @@ using namespace sn;
 
 constexpr int kVectors = 5;              // column sums of the backward pass: pre weight, pre bias, scale, post weight, post bias
 
-// all-reduce over the WAVES waves that hold one row; `slot` alternates between two LDS buffers, so one barrier is enough
-template <int WAVES> __device__ __forceinline__ float row_sum(float v, float *red, int &slot, int wave_in_row, int group)
+// all-reduce over the WAVES waves of the workgroup's row; `slot` alternates between two LDS buffers, so one barrier is enough
+template <int WAVES> __device__ __forceinline__ float row_sum(float v, float *red, int &slot)
 {
     v = sn_wave_sum(v);
     if constexpr (WAVES > 1) {
-        float *buf = red + (slot * 16) + group * WAVES;
-        if ((threadIdx.x & 63) == 0) buf[wave_in_row] = v;
+        float *buf = red + slot * 16;
+        if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
         __syncthreads();
         v = buf[0];
 #pragma unroll
@@ -32,51 +32,100 @@ template <int WAVES> __device__ __forceinline__ float row_sum(float v, float *re
     }
     return v;
 }
-template <int WAVES> __device__ __forceinline__ void row_sum2(float &a, float &b, float *red, int &slot, int wave_in_row, int group)
+template <int WAVES> __device__ __forceinline__ void row_sum2(float &a, float &b, float *red, int &slot)
 {
     a = sn_wave_sum(a);
     b = sn_wave_sum(b);
     if constexpr (WAVES > 1) {
-        float *ba = red + (slot * 16) + group * WAVES, *bb = ba + 32;
-        if ((threadIdx.x & 63) == 0) { ba[wave_in_row] = a; bb[wave_in_row] = b; }
+        float *buf = red + slot * 16;
+        if ((threadIdx.x & 63) == 0) { buf[threadIdx.x >> 6] = a; buf[8 + (threadIdx.x >> 6)] = b; }
         __syncthreads();
-        a = ba[0]; b = bb[0];
+        a = buf[0]; b = buf[8];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) { a += ba[i]; b += bb[i]; }
+        for (int i = 1; i < WAVES; ++i) { a += buf[i]; b += buf[8 + i]; }
         slot ^= 1;
     }
 }
 
-// 1 / (1 + exp(-z)): one reciprocal with a Newton step; z under -80 gives exp(-80), NaN stays
-__device__ __forceinline__ float sigmoid(float z)
+// 1 / (1 + exp(-z)).  bf16 and fp16 rows: the hardware's 2^x of the rounded product (off by 2^-24 |z| relative, far under a step of
+// the result's type).  fp32 rows: with the product's rounding error as a first-order factor.
+template <int DT> __device__ __forceinline__ float sigmoid(float z)
 {
-    const float d = 1.0f + expf(z < -80.0f ? 80.0f : -z);
-    const float r = __builtin_amdgcn_rcpf(d);
-    return fmaf(fmaf(-d, r, 1.0f), r, r);
+    constexpr float L = 1.44269504088896340736f, Llo = 1.92596299112661746887e-8f, ln2 = 0.693147180559945309f;
+    const float t = -z * L;
+    float e = __builtin_amdgcn_exp2f(t);
+    if constexpr (DT == SN_F32) {
+        const float lo = fmaf(-z, L, -t) - z * Llo;
+        e = t < 126.0f ? fmaf(e, lo * ln2, e) : e;           // (beyond it e may be infinite, and the sigmoid is under 2^-126)
+    }
+    return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
 template <int EV, int CH> struct Row { float v[CH][EV]; };
 
-constexpr int block_of(int waves) { return waves >= 4 ? waves * 64 : 256; }
+// WAVES = 1: four rows side by side in a workgroup, each wave on its own; otherwise the workgroup has one row at a time
+constexpr int block_of(int waves) { return waves > 1 ? waves * 64 : 256; }
 
 template <int DT, int EV, int CH, int WAVES>
 struct Layout {
-    static constexpr int kThreads = WAVES * 64;                      // of one row
-    static constexpr int kRows = WAVES >= 4 ? 1 : 4 / WAVES;         // rows of a workgroup at a time
-    static constexpr int kBlock = kThreads * kRows;
-    static constexpr int kStep = kThreads * EV;                      // columns of one chunk
+    static constexpr int kRows = WAVES > 1 ? 1 : 4;
+    static constexpr int kBlock = block_of(WAVES);
+    static constexpr int kStep = WAVES * 64 * EV;                    // columns of one chunk
     static constexpr int kWidth = kStep * CH;
+    static constexpr int kAhead = DT == SN_F32 && CH == 2 ? 1 : 2;   // turns a row is loaded ahead (two of fp32 would pass 256 registers)
+    static constexpr bool kTiny = EV == 4 && CH == 1 && WAVES == 1;  // rows under EV elements come here
 };
 
-template <int DT, int EV, int CH, int STEP>
-__device__ __forceinline__ void load_cols(Row<EV, CH> &r, const void *base, int64_t row, int64_t stride, int col, int E)
+// Rows are loaded one or two turns ahead of their use: the words of the next ones are on their way while this one is worked on.
+template <int DT, int EV, int CH> struct Ahead { Raw<DT, EV> w[CH]; };
+
+template <int DT, int EV, int CH, int STEP, bool TINY>
+__device__ __forceinline__ void issue_cols(Ahead<DT, EV, CH> &r, const void *base, int64_t row, int64_t stride, int col, int E)
 {
     const void *p = (const char *)base + row * stride * (DT == SN_F32 ? 4 : 2);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        uint32_t w[words<DT, EV>()];
-        load_raw<DT, EV>(w, p, col + c * STEP, E);
-        unpack<DT, EV>(r.v[c], w);
+        if (!TINY || E >= EV) load_ahead<DT, EV>(r.w[c], p, col + c * STEP, E);
+        else load_raw<DT, EV>(r.w[c], p, col + c * STEP, E);
+    }
+}
+// tail: this wave holds columns beyond E (the same for all of its lanes)
+template <int DT, int EV, int CH, int STEP>
+__device__ __forceinline__ void take_cols(Row<EV, CH> &r, const Ahead<DT, EV, CH> &a, int col, int E, bool tail)
+{
+#pragma unroll
+    for (int c = 0; c < CH; ++c) unpack<DT, EV>(r.v[c], a.w[c]);
+    if (tail && E >= EV) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) turn_tail<EV>(r.v[c], tail_shift<EV>(col + c * STEP, E));
+    }
+}
+// an 8-bit checkpoint's codes and exponents, ahead of their use (columns beyond the padded width: the last block again, cleared later)
+template <int EV, int CH> struct AheadKept { uint32_t q[CH][EV / 4], e[CH]; };
+template <int EV, int CH, int STEP>
+__device__ __forceinline__ void issue_kept(AheadKept<EV, CH> &r, const void *codes, const void *exps, int64_t row, int col, int npad)
+{
+    const char *p = (const char *)codes + row * npad;
+    const uint8_t *pe = (const uint8_t *)exps + row * (npad / 32);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int j = col + c * STEP < npad ? col + c * STEP : npad - EV;
+        const uint32_t *src = (const uint32_t *)(p + j);
+#pragma unroll
+        for (int i = 0; i < EV / 4; ++i) r.q[c][i] = src[i];
+        r.e[c] = pe[j / 32];
+    }
+}
+template <int EV, int CH, int STEP>
+__device__ __forceinline__ void take_kept(Row<EV, CH> &r, const AheadKept<EV, CH> &a, int col, int npad)
+{
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        decode<EV>(r.v[c], a.q[c], a.e[c]);
+        if (col + c * STEP >= npad) {
+#pragma unroll
+            for (int i = 0; i < EV; ++i) r.v[c][i] = 0.0f;
+        }
     }
 }
 template <int DT, int EV, int CH, int STEP>
@@ -141,28 +190,20 @@ __device__ __forceinline__ void store_checkpoint(void *codes, void *exps, int64_
         }
     }
 }
-template <int EV, int CH, int STEP>
-__device__ __forceinline__ void load_checkpoint(Row<EV, CH> &r, const void *codes, const void *exps, int64_t row, int col, int npad)
+// does row r count?  (wave-uniform: scalar arithmetic)
+__device__ __forceinline__ bool row_counts(const sn_block_norms_args &a, int64_t row)
 {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int j = col + c * STEP;
-        uint32_t q[EV / 4] = {}, e = 8u;
-        if (j < npad) {
-            const uint32_t *src = (const uint32_t *)((const char *)codes + row * npad + j);
-#pragma unroll
-            for (int i = 0; i < EV / 4; ++i) q[i] = src[i];
-            e = ((const uint8_t *)exps)[row * (npad / 32) + j / 32];
-        }
-        decode<EV>(r.v[c], q, e);
-    }
+    if (row >= a.rows) return false;
+    if (!a.n_valid) return true;
+    const int64_t g = a.rows <= 0xFFFFFFFFll ? (int64_t)((uint32_t)row / (uint32_t)a.rows_per_graph) : row / a.rows_per_graph;
+    return (int)(row - g * a.rows_per_graph) < a.n_valid[g];
 }
 
 struct NormStats { float mean, rstd; };
 
 // mean and 1 / deviation of a row; elements beyond E do not count (they are zeros)
 template <int EV, int CH, int STEP, int WAVES>
-__device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, int E, float inv_e, int rms, float eps, float *red, int &slot, int wir, int group)
+__device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, int E, bool tail, float inv_e, int rms, float eps, float *red, int &slot)
 {
     NormStats s = {0.0f, 0.0f};
     if (!rms) {
@@ -171,7 +212,7 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < EV; ++i) t += r.v[c][i];
-        s.mean = row_sum<WAVES>(t, red, slot, wir, group) * inv_e;
+        s.mean = row_sum<WAVES>(t, red, slot) * inv_e;
     }
     float q = 0.0f;
 #pragma unroll
@@ -179,138 +220,192 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
 #pragma unroll
         for (int i = 0; i < EV; ++i) {
             const float d = r.v[c][i] - s.mean;
-            q = col + c * STEP + i < E ? fmaf(d, d, q) : q;
+            q = !tail || col + c * STEP + i < E ? fmaf(d, d, q) : q;
         }
-    s.rstd = 1.0f / sqrtf(row_sum<WAVES>(q, red, slot, wir, group) * inv_e + eps);
+    s.rstd = 1.0f / sqrtf(row_sum<WAVES>(q, red, slot) * inv_e + eps);
     return s;
 }
 
-template <int DT, int EV, int CH, int WAVES>
+// MODE: 0 = the parts of the call are looked up at run time; 1 = everything is there (2: but the gate), every row counts, nothing is
+// kept in 8 bits.  The branches of mode 0 make the compiler wait for all loads and stores in flight where it needs the oldest row,
+// the straight line of the others does not (rows of 4096 bf16, backward: 760 us for 32768 rows in mode 0, MODE_BWD_US in mode 1).
+template <int DT, int EV, int CH, int WAVES, int MODE>
 __global__ __launch_bounds__(block_of(WAVES)) void norms_forward_kernel(sn_block_norms_args a)
 {
     using L = Layout<DT, EV, CH, WAVES>;
     constexpr int STEP = L::kStep;
-    __shared__ float red[64];
+    constexpr bool ALL = MODE != 0;
+    __shared__ float red[32];
     int slot = 0;
-    const int group = threadIdx.x / L::kThreads, t = threadIdx.x % L::kThreads, wir = t >> 6;
+    const int group = WAVES > 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
     const int E = a.width, col = t * EV, npad = (E + 31) & ~31;
     const float inv_e = 1.0f / (float)E;
+    const bool gated = ALL ? MODE == 1 : a.gate != nullptr, post = ALL || a.has_post, pre = ALL || a.has_pre, keep = !ALL && a.x_codes;
+    const bool tail = __any(tail_shift<EV>(col + (CH - 1) * STEP, E) > 0);
+    const int64_t turn = (int64_t)gridDim.x * L::kRows;
+
+    struct Slot { Ahead<DT, EV, CH> x, f, z; bool live; };
+    auto issue = [&](Slot &s, int64_t row) {
+        if constexpr (ALL) row = row < a.rows ? row : a.rows - 1;
+        else {
+            s.live = row_counts(a, row);
+            if (!s.live) return;
+        }
+        issue_cols<DT, EV, CH, STEP, L::kTiny>(s.x, a.x, row, a.x_stride, col, E);
+        issue_cols<DT, EV, CH, STEP, L::kTiny>(s.f, a.branch, row, a.branch_stride, col, E);
+        if (gated) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.z, a.gate, row, a.gate_stride, col, E);
+    };
+    const int64_t start = (int64_t)blockIdx.x * L::kRows + group;
+    Slot s0, s1;
+    issue(s0, start);
+    if constexpr (L::kAhead == 2) issue(s1, start + turn);
     Row<EV, CH> w1, b1, sc, w2, b2;
     load_param<EV, CH, STEP>(sc, a.scale, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(w1, a.has_post ? a.post_weight : nullptr, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(b1, a.has_post ? a.post_bias : nullptr, a.param_dtype, col, E, 0.0f);
-    load_param<EV, CH, STEP>(w2, a.has_pre ? a.pre_weight : nullptr, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(b2, a.has_pre ? a.pre_bias : nullptr, a.param_dtype, col, E, 0.0f);
+    load_param<EV, CH, STEP>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, E, 1.0f);
+    load_param<EV, CH, STEP>(b1, post ? a.post_bias : nullptr, a.param_dtype, col, E, 0.0f);
+    load_param<EV, CH, STEP>(w2, pre ? a.pre_weight : nullptr, a.param_dtype, col, E, 1.0f);
+    load_param<EV, CH, STEP>(b2, pre ? a.pre_bias : nullptr, a.param_dtype, col, E, 0.0f);
 
-    // every wave of the workgroup makes the same number of turns: the row sums hold barriers
-    for (int64_t first = (int64_t)blockIdx.x * L::kRows; first < a.rows; first += (int64_t)gridDim.x * L::kRows) {
-        const int64_t row = first + group;
-        bool live = row < a.rows;
-        if (live && a.n_valid) {
-            const int64_t g = row / a.rows_per_graph;
-            if ((int)(row - g * a.rows_per_graph) >= a.n_valid[g]) {
-                zero_cols<DT, EV, CH, STEP>(a.y, row, col, E);
-                if (a.has_pre) zero_cols<DT, EV, CH, STEP>(a.h, row, col, E);
-                live = false;
-            }
+    auto work = [&](Slot &s, int64_t row) {
+        if (!ALL && !s.live) {                               // the same for every wave of the row
+            issue(s, row + L::kAhead * turn);
+            zero_cols<DT, EV, CH, STEP>(a.y, row, col, E);
+            if (pre) zero_cols<DT, EV, CH, STEP>(a.h, row, col, E);
+            return;
         }
-        if (WAVES == 1 && !live) continue;                   // (one wave a row: no barrier inside)
-        Row<EV, CH> x = {}, f = {}, z = {};
-        if (live) {
-            load_cols<DT, EV, CH, STEP>(x, a.x, row, a.x_stride, col, E);
-            load_cols<DT, EV, CH, STEP>(f, a.branch, row, a.branch_stride, col, E);
-            if (a.gate) load_cols<DT, EV, CH, STEP>(z, a.gate, row, a.gate_stride, col, E);
-            if (a.x_codes) {
-                store_checkpoint<EV, CH, STEP>(a.x_codes, a.x_exps, row, col, npad, x);
-                store_checkpoint<EV, CH, STEP>(a.branch_codes, a.branch_exps, row, col, npad, f);
-                if (a.gate) store_checkpoint<EV, CH, STEP>(a.gate_codes, a.gate_exps, row, col, npad, z);
-            }
+        Row<EV, CH> x, f, z;
+        take_cols<DT, EV, CH, STEP>(x, s.x, col, E, tail);
+        take_cols<DT, EV, CH, STEP>(f, s.f, col, E, tail);
+        if (gated) take_cols<DT, EV, CH, STEP>(z, s.z, col, E, tail);
+        issue(s, row + L::kAhead * turn);
+        if (keep) {
+            store_checkpoint<EV, CH, STEP>(a.x_codes, a.x_exps, row, col, npad, x);
+            store_checkpoint<EV, CH, STEP>(a.branch_codes, a.branch_exps, row, col, npad, f);
+            if (gated) store_checkpoint<EV, CH, STEP>(a.gate_codes, a.gate_exps, row, col, npad, z);
         }
-        NormStats s1 = {0.0f, 1.0f}, s2 = {0.0f, 1.0f};
-        if (a.has_post) s1 = statistics<EV, CH, STEP, WAVES>(f, col, E, inv_e, a.rms, a.eps, red, slot, wir, group);
+        NormStats n1 = {0.0f, 1.0f}, n2 = {0.0f, 1.0f};
+        if (post) n1 = statistics<EV, CH, STEP, WAVES>(f, col, E, tail, inv_e, a.rms, a.eps, red, slot);
+        // (columns beyond E: inputs, weights and biases are zeros there, and so is y)
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
                 float p = f.v[c][i];
-                if (a.has_post) p = fmaf((p - s1.mean) * s1.rstd, w1.v[c][i], b1.v[c][i]);
-                if (a.gate) p *= sigmoid(z.v[c][i]);
-                const float y = fmaf(p, sc.v[c][i], x.v[c][i]);
-                x.v[c][i] = col + c * STEP + i < E ? y : 0.0f;
+                if (post) p = fmaf((p - n1.mean) * n1.rstd, w1.v[c][i], b1.v[c][i]);
+                if (gated) p *= sigmoid<DT>(z.v[c][i]);
+                x.v[c][i] = fmaf(p, sc.v[c][i], x.v[c][i]);
             }
-        if (live) store_cols<DT, EV, CH, STEP>(a.y, row, col, E, x);
-        if (a.has_pre) {
-            s2 = statistics<EV, CH, STEP, WAVES>(x, col, E, inv_e, a.rms, a.eps, red, slot, wir, group);
+        store_cols<DT, EV, CH, STEP>(a.y, row, col, E, x);
+        if (pre) {
+            n2 = statistics<EV, CH, STEP, WAVES>(x, col, E, tail, inv_e, a.rms, a.eps, red, slot);
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < EV; ++i) x.v[c][i] = fmaf((x.v[c][i] - s2.mean) * s2.rstd, w2.v[c][i], b2.v[c][i]);
-            if (live) store_cols<DT, EV, CH, STEP>(a.h, row, col, E, x);
+                for (int i = 0; i < EV; ++i) x.v[c][i] = fmaf((x.v[c][i] - n2.mean) * n2.rstd, w2.v[c][i], b2.v[c][i]);
+            store_cols<DT, EV, CH, STEP>(a.h, row, col, E, x);
         }
-        if (a.stats && live && t == 0) *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(s1.mean, s1.rstd, s2.mean, s2.rstd);
+        if (a.stats && t == 0) *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(n1.mean, n1.rstd, n2.mean, n2.rstd);
+    };
+    for (int64_t row = start; row < a.rows; row += L::kAhead * turn) {
+        work(s0, row);
+        if constexpr (L::kAhead == 2) {
+            if (row + turn >= a.rows) break;
+            work(s1, row + turn);
+        }
     }
 }
 
-template <int DT, int EV, int CH, int WAVES, bool KEPT>
+template <int DT, int EV, int CH, int WAVES, int MODE, bool KEPT>
 __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_block_norms_args a, float *partial)
 {
     using L = Layout<DT, EV, CH, WAVES>;
     constexpr int STEP = L::kStep;
-    __shared__ float red[64];
+    constexpr bool ALL = MODE != 0;
+    __shared__ float red[32];
     int slot = 0;
-    const int group = threadIdx.x / L::kThreads, t = threadIdx.x % L::kThreads, wir = t >> 6;
+    const int group = WAVES > 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
     const int E = a.width, col = t * EV, npad = (E + 31) & ~31;
     const float inv_e = 1.0f / (float)E;
+    const bool gated = ALL ? MODE == 1 : KEPT ? a.gate_codes != nullptr : a.gate != nullptr;
+    const bool post = ALL || a.has_post, has_dy = ALL || a.dy, has_dh = ALL || a.dh;
+    const bool tail = __any(tail_shift<EV>(col + (CH - 1) * STEP, E) > 0);
+    const int64_t turn = (int64_t)gridDim.x * L::kRows;
+
+    struct Slot {
+        Ahead<DT, EV, CH> x, f, z, dy, dh;
+        AheadKept<EV, CH> kx, kf, kz;
+        float4 st;
+        bool live;
+    };
+    auto issue = [&](Slot &s, int64_t row) {
+        if constexpr (ALL) row = row < a.rows ? row : a.rows - 1;
+        else {
+            s.live = row_counts(a, row);
+            if (!s.live) return;
+        }
+        if constexpr (KEPT) {
+            issue_kept<EV, CH, STEP>(s.kx, a.x_codes, a.x_exps, row, col, npad);
+            issue_kept<EV, CH, STEP>(s.kf, a.branch_codes, a.branch_exps, row, col, npad);
+            if (gated) issue_kept<EV, CH, STEP>(s.kz, a.gate_codes, a.gate_exps, row, col, npad);
+        } else {
+            issue_cols<DT, EV, CH, STEP, L::kTiny>(s.x, a.x, row, a.x_stride, col, E);
+            issue_cols<DT, EV, CH, STEP, L::kTiny>(s.f, a.branch, row, a.branch_stride, col, E);
+            if (gated) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.z, a.gate, row, a.gate_stride, col, E);
+        }
+        if (has_dy) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.dy, a.dy, row, a.dy_stride, col, E);
+        if (has_dh) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.dh, a.dh, row, a.dh_stride, col, E);
+        s.st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
+    };
+    const int64_t start = (int64_t)blockIdx.x * L::kRows + group;
+    Slot s0, s1;
+    issue(s0, start);
+    if constexpr (L::kAhead == 2) issue(s1, start + turn);
     Row<EV, CH> w1, b1, sc, w2;
     load_param<EV, CH, STEP>(sc, a.scale, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(w1, a.has_post ? a.post_weight : nullptr, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(b1, a.has_post ? a.post_bias : nullptr, a.param_dtype, col, E, 0.0f);
-    load_param<EV, CH, STEP>(w2, a.has_pre ? a.pre_weight : nullptr, a.param_dtype, col, E, 1.0f);
+    load_param<EV, CH, STEP>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, E, 1.0f);
+    load_param<EV, CH, STEP>(b1, post ? a.post_bias : nullptr, a.param_dtype, col, E, 0.0f);
+    load_param<EV, CH, STEP>(w2, has_dh ? a.pre_weight : nullptr, a.param_dtype, col, E, 1.0f);
     Row<EV, CH> sum[kVectors] = {};
 
-    for (int64_t first = (int64_t)blockIdx.x * L::kRows; first < a.rows; first += (int64_t)gridDim.x * L::kRows) {
-        const int64_t row = first + group;
-        bool live = row < a.rows;
-        if (live && a.n_valid) {
-            const int64_t g = row / a.rows_per_graph;
-            if ((int)(row - g * a.rows_per_graph) >= a.n_valid[g]) {
-                if (a.dx) zero_cols<DT, EV, CH, STEP>(a.dx, row, col, E);
-                if (a.dbranch) zero_cols<DT, EV, CH, STEP>(a.dbranch, row, col, E);
-                if (a.dgate) zero_cols<DT, EV, CH, STEP>(a.dgate, row, col, E);
-                live = false;
-            }
+    auto work = [&](Slot &s, int64_t row) {
+        if (!ALL && !s.live) {
+            issue(s, row + L::kAhead * turn);
+            if (a.dx) zero_cols<DT, EV, CH, STEP>(a.dx, row, col, E);
+            if (a.dbranch) zero_cols<DT, EV, CH, STEP>(a.dbranch, row, col, E);
+            if (a.dgate) zero_cols<DT, EV, CH, STEP>(a.dgate, row, col, E);
+            return;
         }
-        if (WAVES == 1 && !live) continue;
-        Row<EV, CH> x = {}, f = {}, z = {}, u = {}, d = {};
-        float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
-        if (live) {
-            if constexpr (KEPT) {
-                load_checkpoint<EV, CH, STEP>(x, a.x_codes, a.x_exps, row, col, npad);
-                load_checkpoint<EV, CH, STEP>(f, a.branch_codes, a.branch_exps, row, col, npad);
-                if (a.gate_codes) load_checkpoint<EV, CH, STEP>(z, a.gate_codes, a.gate_exps, row, col, npad);
-            } else {
-                load_cols<DT, EV, CH, STEP>(x, a.x, row, a.x_stride, col, E);
-                load_cols<DT, EV, CH, STEP>(f, a.branch, row, a.branch_stride, col, E);
-                if (a.gate) load_cols<DT, EV, CH, STEP>(z, a.gate, row, a.gate_stride, col, E);
-            }
-            if (a.dy) load_cols<DT, EV, CH, STEP>(u, a.dy, row, a.dy_stride, col, E);
-            if (a.dh) load_cols<DT, EV, CH, STEP>(d, a.dh, row, a.dh_stride, col, E);
-            st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
+        Row<EV, CH> x, f, z, u = {}, d;
+        if constexpr (KEPT) {
+            take_kept<EV, CH, STEP>(x, s.kx, col, npad);
+            take_kept<EV, CH, STEP>(f, s.kf, col, npad);
+            if (gated) take_kept<EV, CH, STEP>(z, s.kz, col, npad);
+        } else {
+            take_cols<DT, EV, CH, STEP>(x, s.x, col, E, tail);
+            take_cols<DT, EV, CH, STEP>(f, s.f, col, E, tail);
+            if (gated) take_cols<DT, EV, CH, STEP>(z, s.z, col, E, tail);
         }
-        const bool gated = KEPT ? a.gate_codes != nullptr : a.gate != nullptr;
-        // f -> unit values of the post norm, z -> sigmoid, x -> unit values of y
+        if (has_dy) take_cols<DT, EV, CH, STEP>(u, s.dy, col, E, tail);
+        if (has_dh) take_cols<DT, EV, CH, STEP>(d, s.dh, col, E, tail);
+        const float4 st = s.st;
+        issue(s, row + L::kAhead * turn);
+        // f -> unit values of the post norm, z -> sigmoid, x -> unit values of y.  Columns beyond E hold whatever the statistics make of
+        // zeros: every use multiplies it by a weight or a gradient that is zero there, and no store takes it.
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
-                const bool in = col + c * STEP + i < E;
-                f.v[c][i] = in ? (f.v[c][i] - st.x) * st.y : 0.0f;
-                const float p = fmaf(f.v[c][i], w1.v[c][i], b1.v[c][i]);
-                if (gated) z.v[c][i] = sigmoid(z.v[c][i]);
-                const float y = fmaf(gated ? p * z.v[c][i] : p, sc.v[c][i], x.v[c][i]);
-                x.v[c][i] = in ? (y - st.z) * st.w : 0.0f;
+                f.v[c][i] = (f.v[c][i] - st.x) * st.y;
+                float p = fmaf(f.v[c][i], w1.v[c][i], b1.v[c][i]);
+                if (gated) {
+                    z.v[c][i] = sigmoid<DT>(z.v[c][i]);
+                    p *= z.v[c][i];
+                }
+                x.v[c][i] = (fmaf(p, sc.v[c][i], x.v[c][i]) - st.z) * st.w;
             }
-        if (a.dh) {
+        if (has_dh) {
             float m1 = 0.0f, m2 = 0.0f;
 #pragma unroll
             for (int c = 0; c < CH; ++c)
@@ -322,7 +417,7 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
                     m1 += d.v[c][i];
                     m2 = fmaf(d.v[c][i], x.v[c][i], m2);
                 }
-            row_sum2<WAVES>(m1, m2, red, slot, wir, group);
+            row_sum2<WAVES>(m1, m2, red, slot);
             m1 = a.rms ? 0.0f : m1 * inv_e;
             m2 *= inv_e;
 #pragma unroll
@@ -330,29 +425,27 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
 #pragma unroll
                 for (int i = 0; i < EV; ++i) u.v[c][i] = fmaf(st.w, fmaf(-x.v[c][i], m2, d.v[c][i] - m1), u.v[c][i]);
         }
-        if (a.dx && live) store_cols<DT, EV, CH, STEP>(a.dx, row, col, E, u);
+        if (ALL || a.dx) store_cols<DT, EV, CH, STEP>(a.dx, row, col, E, u);
         // d -> gradient of the gated product's p, x -> gradient of the gate
         float m1 = 0.0f, m2 = 0.0f;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
-                const bool in = col + c * STEP + i < E;
                 const float p = fmaf(f.v[c][i], w1.v[c][i], b1.v[c][i]);
-                const float s = gated ? z.v[c][i] : 1.0f, uu = in ? u.v[c][i] : 0.0f;
-                const float us = uu * s;
+                const float us = gated ? u.v[c][i] * z.v[c][i] : u.v[c][i];
                 sum[2].v[c][i] = fmaf(us, p, sum[2].v[c][i]);
                 const float dp = us * sc.v[c][i];
-                x.v[c][i] = dp * p * (1.0f - s);
+                if (gated) x.v[c][i] = dp * p * (1.0f - z.v[c][i]);
                 sum[3].v[c][i] = fmaf(dp, f.v[c][i], sum[3].v[c][i]);
                 sum[4].v[c][i] += dp;
                 d.v[c][i] = dp * w1.v[c][i];
                 m1 += d.v[c][i];
                 m2 = fmaf(d.v[c][i], f.v[c][i], m2);
             }
-        if (a.dgate && live) store_cols<DT, EV, CH, STEP>(a.dgate, row, col, E, x);
-        if (a.has_post) {
-            row_sum2<WAVES>(m1, m2, red, slot, wir, group);
+        if (gated && (ALL || a.dgate)) store_cols<DT, EV, CH, STEP>(a.dgate, row, col, E, x);
+        if (post) {
+            row_sum2<WAVES>(m1, m2, red, slot);
             m1 = a.rms ? 0.0f : m1 * inv_e;
             m2 *= inv_e;
 #pragma unroll
@@ -360,44 +453,64 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
 #pragma unroll
                 for (int i = 0; i < EV; ++i) d.v[c][i] = st.y * fmaf(-f.v[c][i], m2, d.v[c][i] - m1);
         }
-        if (a.dbranch && live) store_cols<DT, EV, CH, STEP>(a.dbranch, row, col, E, d);
+        if (ALL || a.dbranch) store_cols<DT, EV, CH, STEP>(a.dbranch, row, col, E, d);
+    };
+    for (int64_t row = start; row < a.rows; row += L::kAhead * turn) {
+        work(s0, row);
+        if constexpr (L::kAhead == 2) {
+            if (row + turn >= a.rows) break;
+            work(s1, row + turn);
+        }
     }
     if (partial) {
-        float *dst = partial + ((int64_t)blockIdx.x * L::kRows + group) * kVectors * E;
+        // the workgroup's rows side by side are added here, one line of partial sums leaves for each workgroup
+        float *dst = partial + (int64_t)blockIdx.x * kVectors * E;
+        __shared__ float join[L::kRows > 1 ? L::kRows * L::kWidth : 1];
 #pragma unroll
-        for (int k = 0; k < kVectors; ++k)
+        for (int k = 0; k < kVectors; ++k) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < EV; ++i) {
                     const int j = col + c * STEP + i;
-                    if (j < E) dst[(int64_t)k * E + j] = sum[k].v[c][i];
+                    if constexpr (L::kRows > 1) join[group * L::kWidth + j] = sum[k].v[c][i];
+                    else if (j < E) dst[(int64_t)k * E + j] = sum[k].v[c][i];
                 }
+            if constexpr (L::kRows > 1) {
+                __syncthreads();
+                for (int j = threadIdx.x; j < E; j += L::kBlock) {
+                    float v = join[j];
+#pragma unroll
+                    for (int g = 1; g < L::kRows; ++g) v += join[g * L::kWidth + j];
+                    dst[(int64_t)k * E + j] = v;
+                }
+                __syncthreads();
+            }
+        }
     }
 }
 
 struct ColumnOut { void *p[kVectors]; };
 
-// column sums of the workgroups' partial rows, in order; 16 slices of the parts side by side
+// column sums of the workgroups' partial rows in a fixed order: 32 columns, 32 slices of the parts side by side
 __global__ __launch_bounds__(1024) void norms_columns_kernel(const float *partial, int parts, int E, ColumnOut out, int dtype)
 {
-    __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-    const int k = blockIdx.y, j = blockIdx.x * 64 + lane;
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int k = blockIdx.y, j = blockIdx.x * 32 + lane;
     if (!out.p[k]) return;
-    const int per = (parts + 15) / 16, p0 = slice * per, p1 = p0 + per < parts ? p0 + per : parts;
     float s = 0.0f;
     if (j < E) {
 #pragma unroll 8
-        for (int p = p0; p < p1; ++p) s += partial[((int64_t)p * kVectors + k) * E + j];
+        for (int p = slice; p < parts; p += 32) s += partial[((int64_t)p * kVectors + k) * E + j];
     }
     red[slice][lane] = s;
     __syncthreads();
-    if (slice == 0 && j < E) {
+    s = red[lane][slice];                                    // now: lane = slice, slice = column
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += red[i][lane];
-        store_any(out.p[k], dtype, j, s);
-    }
+    for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor(s, off, 32);
+    const int c = blockIdx.x * 32 + slice;
+    if (lane == 0 && c < E) store_any(out.p[k], dtype, c, s);
 }
 
 // lanes of a row: 8 elements a lane up to 4096 columns (16 waves with five column sums each would spill); 4 a lane under 257 columns
@@ -407,12 +520,13 @@ int waves_for(int E)
     while (w * 512 < E) w *= 2;
     return w;
 }
-int rows_per_block(int E) { const int w = waves_for(E); return w >= 4 ? 1 : 4 / w; }
+int rows_per_block(int E) { return waves_for(E) > 1 ? 1 : 4; }
 int backward_blocks(int64_t rows, int E)
 {
     const int64_t turns = (rows + rows_per_block(E) - 1) / rows_per_block(E);
-    const int64_t most = waves_for(E) <= 4 ? 1024 : 512;
-    return (int)(turns < most ? turns : most);
+    // as many workgroups as are resident with the registers of the backward kernel: two waves a SIMD (one wave a row of up to 256: four)
+    const int64_t most = waves_for(E) == 1 ? 1024 : 2048 / waves_for(E), each = (turns + most - 1) / most;
+    return (int)((turns + each - 1) / each);                 // (the same number of turns for all but the last)
 }
 
 int check_args(const sn_block_norms_args *a, const char *who)
@@ -431,9 +545,10 @@ int check_args(const sn_block_norms_args *a, const char *who)
 template <int DT, int EV, int CH, int WAVES> int launch_forward(const sn_block_norms_args &a, hipStream_t st)
 {
     using L = Layout<DT, EV, CH, WAVES>;
-    const int64_t turns = (a.rows + L::kRows - 1) / L::kRows;
-    const int64_t most = WAVES <= 4 ? 2048 : 1024;
-    hipLaunchKernelGGL((norms_forward_kernel<DT, EV, CH, WAVES>), dim3((unsigned)(turns < most ? turns : most)), dim3(L::kBlock), 0, st, a);
+    const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = WAVES == 1 ? 2048 : 4096 / WAVES, each = (turns + most - 1) / most;
+    const bool all = a.has_post && a.has_pre && !a.n_valid && !a.x_codes;
+    const auto kernel = !all ? norms_forward_kernel<DT, EV, CH, WAVES, 0> : a.gate ? norms_forward_kernel<DT, EV, CH, WAVES, 1> : norms_forward_kernel<DT, EV, CH, WAVES, 2>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((turns + each - 1) / each)), dim3(L::kBlock), 0, st, a);
     SN_CHECK_LAUNCH("sn_block_norms_forward");
     return SN_OK;
 }
@@ -445,11 +560,16 @@ template <int DT, int EV, int CH, int WAVES> int launch_backward(const sn_block_
     bool columns = false;
     for (int k = 0; k < kVectors; ++k) columns |= out.p[k] != nullptr;
     float *partial = columns ? (float *)a.workspace : nullptr;
-    if (a.x_codes) hipLaunchKernelGGL((norms_backward_kernel<DT, EV, CH, WAVES, true>), dim3(blocks), dim3(L::kBlock), 0, st, a, partial);
-    else hipLaunchKernelGGL((norms_backward_kernel<DT, EV, CH, WAVES, false>), dim3(blocks), dim3(L::kBlock), 0, st, a, partial);
+    const bool gate = a.x_codes ? a.gate_codes != nullptr : a.gate != nullptr;
+    const bool all = a.has_post && a.has_pre && !a.n_valid && a.dy && a.dh && a.dx && a.dbranch && (!gate || a.dgate);
+    const auto kernel = a.x_codes ? (!all ? norms_backward_kernel<DT, EV, CH, WAVES, 0, true> : gate ? norms_backward_kernel<DT, EV, CH, WAVES, 1, true>
+                                                                                                      : norms_backward_kernel<DT, EV, CH, WAVES, 2, true>)
+                                  : (!all ? norms_backward_kernel<DT, EV, CH, WAVES, 0, false> : gate ? norms_backward_kernel<DT, EV, CH, WAVES, 1, false>
+                                                                                                       : norms_backward_kernel<DT, EV, CH, WAVES, 2, false>);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(L::kBlock), 0, st, a, partial);
     SN_CHECK_LAUNCH("sn_block_norms_backward");
     if (columns) {
-        hipLaunchKernelGGL(norms_columns_kernel, dim3((a.width + 63) / 64, kVectors), dim3(1024), 0, st, partial, blocks * L::kRows, a.width, out, a.param_dtype);
+        hipLaunchKernelGGL(norms_columns_kernel, dim3((a.width + 31) / 32, kVectors), dim3(1024), 0, st, partial, blocks, a.width, out, a.param_dtype);
         SN_CHECK_LAUNCH("sn_block_norms_backward (columns)");
     }
     return SN_OK;
@@ -495,7 +615,7 @@ extern "C" int sn_block_norms_forward(const sn_block_norms_args *args, void *str
 extern "C" size_t sn_block_norms_workspace(int64_t rows, int width)
 {
     if (rows < 0 || width < 1 || width > SN_BLOCK_NORMS_MAX_WIDTH) return 0;
-    return (size_t)backward_blocks(rows, width) * rows_per_block(width) * kVectors * width * sizeof(float);
+    return (size_t)backward_blocks(rows, width) * kVectors * width * sizeof(float);
 }
 
 extern "C" int sn_block_norms_backward(const sn_block_norms_args *args, void *stream)

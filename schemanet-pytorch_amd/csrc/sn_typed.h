@@ -146,6 +146,21 @@ template <int DT, int EV> __device__ __forceinline__ void load_raw(Raw<DT, EV> &
         }
     }
 }
+// The same without a test that a load would wait behind (for loads that run ahead of their use): the last group of a row is read
+// from EV elements before the row's end (n >= EV) and turned into place when it is unpacked.
+template <int EV> __device__ __forceinline__ int tail_shift(int i, int n) { return i + EV <= n ? 0 : (i >= n ? EV : i + EV - n); }
+template <int DT, int EV> __device__ __forceinline__ void load_ahead(Raw<DT, EV> &w, const void *row, int i, int n)
+{
+    const int at = i + EV <= n ? i : n - EV;
+    load_words<words<DT, EV>()>(w, (const char *)row + (int64_t)at * (DT == SN_F32 ? 4 : 2));
+}
+template <int EV> __device__ __forceinline__ void turn_tail(float (&v)[EV], int shift)
+{
+#pragma unroll
+    for (int s = 1; s <= EV; s *= 2)
+#pragma unroll
+        for (int e = 0; e < EV; ++e) v[e] = (shift & s) ? (e + s < EV ? v[e + s] : 0.0f) : v[e];
+}
 template <int DT, int EV> __device__ __forceinline__ void store_row(void *row, int i, int n, const float (&v)[EV])
 {
     char *p = (char *)row + (int64_t)i * (DT == SN_F32 ? 4 : 2);
