@@ -86,9 +86,11 @@ int sn_block_norms_backward(const sn_block_norms_args *args, void *stream);
  * logits [rows, n]; target [rows] int64.  p = softmax(logits).
  *   log_probs[r] = log p[target], 0 where target == ignore_index, NaN where the target is outside 0 .. n - 1;
  *   entropy[r] = -sum p log p;   top_ids / top_log_probs [rows, k]: the k largest, the lowest index first among equals
- *   stats [rows, 3]: max, sum of exp(x - max), entropy - what the backward pass reads.
+ *   stats [rows, 3]: max, sum of exp(x - max), entropy - what the backward pass reads (NULL: not wanted).
+ *   workspace: sn_label_log_probs_workspace bytes (0: none needed, NULL will do).
  * A row whose every logit is -inf has no distribution: log_probs -inf, entropy 0, gradient 0.  A NaN or +inf logit makes the
- * row's outputs NaN (the ids are then those of the largest logits that are not NaN, -1 where there are fewer than k).
+ * row's outputs NaN (the ids are then those of the largest finite or +inf logits, -1 where there are
+ * fewer than k).
  * ------------------------------------------------------------------------------------------ */
 #define SN_SCORES_MAX_TOP 64
 size_t sn_label_log_probs_workspace(int64_t rows, int64_t n, int k);

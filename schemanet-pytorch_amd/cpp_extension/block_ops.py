@@ -387,20 +387,20 @@ def gated_residual_norms(x, branch, gate=None, scale=None, post=None, pre=None, 
 LabelLogProbs = namedtuple("LabelLogProbs", ["log_probs", "entropy", "top_log_probs", "top_ids"])
 
 
-def _scores_forward(logits, target, ignore_index, topk):
+def _scores_forward(logits, target, ignore_index, topk, train):
     lib = _library()
     dev, n = logits.device, logits.shape[-1]
     lead = target.shape
     rows = target.numel()
     f32 = dict(dtype=torch.float32, device=dev)
     lp, ent = torch.empty(lead, **f32), torch.empty(lead, **f32)
-    stats = torch.empty((rows, 3), **f32)             # what the backward pass reads
+    stats = torch.empty((rows, 3), **f32) if train else None             # what the backward pass reads
     top_lp = torch.empty((*lead, topk), **f32) if topk else None
     top_ids = torch.empty((*lead, topk), dtype=torch.int64, device=dev) if topk else None
     if rows:
         v, stride = _rows(logits, n)
         size = lib.sn_label_log_probs_workspace(rows, n, topk)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _launch(lib.sn_label_log_probs, "sn_label_log_probs", dev, _p(v), _TYPES[logits.dtype], rows, n, stride, _p(target), ignore_index, topk, _p(lp), _p(ent),
                 _p(stats), _p(top_lp), _p(top_ids), _p(ws), size)
     return lp, ent, stats, top_lp, top_ids
@@ -410,7 +410,7 @@ class _LabelLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, ignore_index, topk):
         logits = logits.detach()
-        lp, ent, stats, top_lp, top_ids = _scores_forward(logits, target, ignore_index, topk)
+        lp, ent, stats, top_lp, top_ids = _scores_forward(logits, target, ignore_index, topk, True)
         ctx.save_for_backward(logits, target, stats)
         ctx.ignore_index = ignore_index
         ctx.set_materialize_grads(False)
@@ -457,5 +457,5 @@ def label_log_probs(logits, target, topk=0, ignore_index=-100):
     if _wants_grad(logits):
         out = _LabelLogProbs.apply(logits, target, int(ignore_index), topk)
         return LabelLogProbs(*out) if topk else LabelLogProbs(*out, None, None)
-    lp, ent, _, top_lp, top_ids = _scores_forward(logits, target, int(ignore_index), topk)
+    lp, ent, _, top_lp, top_ids = _scores_forward(logits, target, int(ignore_index), topk, False)
     return LabelLogProbs(lp, ent, top_lp, top_ids)

@@ -17,32 +17,33 @@ using namespace sn;
 
 constexpr int kVectors = 5;              // column sums of the backward pass: pre weight, pre bias, scale, post weight, post bias
 
-// all-reduce over the WAVES waves of the workgroup's row; `slot` alternates between two LDS buffers, so one barrier is enough
-template <int WAVES> __device__ __forceinline__ float row_sum(float v, float *red, int &slot)
+// all-reduce over the waves of the workgroup's row (up to 8; the buffers hold zeros for those that are not there); `slot` alternates
+// between two LDS buffers, so one barrier is enough
+template <bool MULTI> __device__ __forceinline__ float row_sum(float v, float *red, int &slot)
 {
     v = sn_wave_sum(v);
-    if constexpr (WAVES > 1) {
+    if constexpr (MULTI) {
         float *buf = red + slot * 16;
         if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = buf[0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) v += buf[i];
+        const float4 a = *reinterpret_cast<const float4 *>(buf), b = *reinterpret_cast<const float4 *>(buf + 4);
+        v = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
         slot ^= 1;
     }
     return v;
 }
-template <int WAVES> __device__ __forceinline__ void row_sum2(float &a, float &b, float *red, int &slot)
+template <bool MULTI> __device__ __forceinline__ void row_sum2(float &p, float &q, float *red, int &slot)
 {
-    a = sn_wave_sum(a);
-    b = sn_wave_sum(b);
-    if constexpr (WAVES > 1) {
+    p = sn_wave_sum(p);
+    q = sn_wave_sum(q);
+    if constexpr (MULTI) {
         float *buf = red + slot * 16;
-        if ((threadIdx.x & 63) == 0) { buf[threadIdx.x >> 6] = a; buf[8 + (threadIdx.x >> 6)] = b; }
+        if ((threadIdx.x & 63) == 0) { buf[threadIdx.x >> 6] = p; buf[8 + (threadIdx.x >> 6)] = q; }
         __syncthreads();
-        a = buf[0]; b = buf[8];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) { a += buf[i]; b += buf[8 + i]; }
+        const float4 a = *reinterpret_cast<const float4 *>(buf), b = *reinterpret_cast<const float4 *>(buf + 4);
+        const float4 c = *reinterpret_cast<const float4 *>(buf + 8), d = *reinterpret_cast<const float4 *>(buf + 12);
+        p = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+        q = ((c.x + c.y) + (c.z + c.w)) + ((d.x + d.y) + (d.z + d.w));
         slot ^= 1;
     }
 }
@@ -63,101 +64,101 @@ template <int DT> __device__ __forceinline__ float sigmoid(float z)
 
 template <int EV, int CH> struct Row { float v[CH][EV]; };
 
-// WAVES = 1: four rows side by side in a workgroup, each wave on its own; otherwise the workgroup has one row at a time
-constexpr int block_of(int waves) { return waves > 1 ? waves * 64 : 256; }
+// MULTI: the workgroup's 2 .. 8 waves have one row at a time; otherwise four rows side by side, each wave on its own
+constexpr int block_of(bool multi) { return multi ? 512 : 256; }
 
-template <int DT, int EV, int CH, int WAVES>
+template <int DT, int EV, int CH, bool MULTI>
 struct Layout {
-    static constexpr int kRows = WAVES > 1 ? 1 : 4;
-    static constexpr int kBlock = block_of(WAVES);
-    static constexpr int kStep = WAVES * 64 * EV;                    // columns of one chunk
-    static constexpr int kWidth = kStep * CH;
-    static constexpr int kAhead = DT == SN_F32 && CH == 2 ? 1 : 2;   // turns a row is loaded ahead (two of fp32 would pass 256 registers)
-    static constexpr bool kTiny = EV == 4 && CH == 1 && WAVES == 1;  // rows under EV elements come here
+    static constexpr int kRows = MULTI ? 1 : 4;
+    static constexpr int kWidth = 64 * EV * CH;                      // of one wave
+    // turns a row is loaded ahead: two where the registers allow it.  fp32, 103424 rows of 256: forward 120 us with one, 110 with
+    // two; backward 162 with one, 210 with two (a fourth of the waves less)
+    static constexpr int kAheadForward = DT == SN_F32 && CH == 2 ? 1 : 2, kAheadBackward = DT == SN_F32 ? 1 : 2;
+    static constexpr bool kTiny = EV == 4 && CH == 1 && !MULTI;      // rows under EV elements come here
 };
 
 // Rows are loaded one or two turns ahead of their use: the words of the next ones are on their way while this one is worked on.
 template <int DT, int EV, int CH> struct Ahead { Raw<DT, EV> w[CH]; };
 
-template <int DT, int EV, int CH, int STEP, bool TINY>
-__device__ __forceinline__ void issue_cols(Ahead<DT, EV, CH> &r, const void *base, int64_t row, int64_t stride, int col, int E)
+template <int DT, int EV, int CH, bool TINY>
+__device__ __forceinline__ void issue_cols(Ahead<DT, EV, CH> &r, const void *base, int64_t row, int64_t stride, int col, int step, int E)
 {
     const void *p = (const char *)base + row * stride * (DT == SN_F32 ? 4 : 2);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        if (!TINY || E >= EV) load_ahead<DT, EV>(r.w[c], p, col + c * STEP, E);
-        else load_raw<DT, EV>(r.w[c], p, col + c * STEP, E);
+        if (!TINY || E >= EV) load_ahead<DT, EV>(r.w[c], p, col + c * step, E);
+        else load_raw<DT, EV>(r.w[c], p, col + c * step, E);
     }
 }
 // tail: this wave holds columns beyond E (the same for all of its lanes)
-template <int DT, int EV, int CH, int STEP>
-__device__ __forceinline__ void take_cols(Row<EV, CH> &r, const Ahead<DT, EV, CH> &a, int col, int E, bool tail)
+template <int DT, int EV, int CH>
+__device__ __forceinline__ void take_cols(Row<EV, CH> &r, const Ahead<DT, EV, CH> &a, int col, int step, int E, bool tail)
 {
 #pragma unroll
     for (int c = 0; c < CH; ++c) unpack<DT, EV>(r.v[c], a.w[c]);
     if (tail && E >= EV) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) turn_tail<EV>(r.v[c], tail_shift<EV>(col + c * STEP, E));
+        for (int c = 0; c < CH; ++c) turn_tail<EV>(r.v[c], tail_shift<EV>(col + c * step, E));
     }
 }
 // an 8-bit checkpoint's codes and exponents, ahead of their use (columns beyond the padded width: the last block again, cleared later)
 template <int EV, int CH> struct AheadKept { uint32_t q[CH][EV / 4], e[CH]; };
-template <int EV, int CH, int STEP>
-__device__ __forceinline__ void issue_kept(AheadKept<EV, CH> &r, const void *codes, const void *exps, int64_t row, int col, int npad)
+template <int EV, int CH>
+__device__ __forceinline__ void issue_kept(AheadKept<EV, CH> &r, const void *codes, const void *exps, int64_t row, int col, int step, int npad)
 {
     const char *p = (const char *)codes + row * npad;
     const uint8_t *pe = (const uint8_t *)exps + row * (npad / 32);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int j = col + c * STEP < npad ? col + c * STEP : npad - EV;
+        const int j = col + c * step < npad ? col + c * step : npad - EV;
         const uint32_t *src = (const uint32_t *)(p + j);
 #pragma unroll
         for (int i = 0; i < EV / 4; ++i) r.q[c][i] = src[i];
         r.e[c] = pe[j / 32];
     }
 }
-template <int EV, int CH, int STEP>
-__device__ __forceinline__ void take_kept(Row<EV, CH> &r, const AheadKept<EV, CH> &a, int col, int npad)
+template <int EV, int CH>
+__device__ __forceinline__ void take_kept(Row<EV, CH> &r, const AheadKept<EV, CH> &a, int col, int step, int npad)
 {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         decode<EV>(r.v[c], a.q[c], a.e[c]);
-        if (col + c * STEP >= npad) {
+        if (col + c * step >= npad) {
 #pragma unroll
             for (int i = 0; i < EV; ++i) r.v[c][i] = 0.0f;
         }
     }
 }
-template <int DT, int EV, int CH, int STEP>
-__device__ __forceinline__ void store_cols(void *base, int64_t row, int col, int E, const Row<EV, CH> &r)
+template <int DT, int EV, int CH>
+__device__ __forceinline__ void store_cols(void *base, int64_t row, int col, int step, int E, const Row<EV, CH> &r)
 {
     void *p = (char *)base + row * E * (DT == SN_F32 ? 4 : 2);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) store_row<DT, EV>(p, col + c * STEP, E, r.v[c]);
+    for (int c = 0; c < CH; ++c) store_row<DT, EV>(p, col + c * step, E, r.v[c]);
 }
-template <int DT, int EV, int CH, int STEP>
-__device__ __forceinline__ void zero_cols(void *base, int64_t row, int col, int E)
+template <int DT, int EV, int CH>
+__device__ __forceinline__ void zero_cols(void *base, int64_t row, int col, int step, int E)
 {
     Row<EV, CH> z;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int i = 0; i < EV; ++i) z.v[c][i] = 0.0f;
-    store_cols<DT, EV, CH, STEP>(base, row, col, E, z);
+    store_cols<DT, EV, CH>(base, row, col, step, E, z);
 }
-template <int PT, int EV, int CH, int STEP>
-__device__ __forceinline__ void load_param_as(Row<EV, CH> &r, const void *p, int col, int E)
+template <int PT, int EV, int CH>
+__device__ __forceinline__ void load_param_as(Row<EV, CH> &r, const void *p, int col, int step, int E)
 {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         Raw<PT, EV> w;
-        load_raw<PT, EV>(w, p, col + c * STEP, E);
+        load_raw<PT, EV>(w, p, col + c * step, E);
         unpack<PT, EV>(r.v[c], w);
     }
 }
 // (columns beyond E get zeros)
-template <int EV, int CH, int STEP>
-__device__ __forceinline__ void load_param(Row<EV, CH> &r, const void *p, int dtype, int col, int E, float none)
+template <int EV, int CH>
+__device__ __forceinline__ void load_param(Row<EV, CH> &r, const void *p, int dtype, int col, int step, int E, float none)
 {
     if (!p) {
 #pragma unroll
@@ -165,20 +166,20 @@ __device__ __forceinline__ void load_param(Row<EV, CH> &r, const void *p, int dt
 #pragma unroll
             for (int i = 0; i < EV; ++i) r.v[c][i] = none;
     } else if (dtype == SN_F32) {
-        load_param_as<SN_F32, EV, CH, STEP>(r, p, col, E);
+        load_param_as<SN_F32, EV, CH>(r, p, col, step, E);
     } else if (dtype == SN_BF16) {
-        load_param_as<SN_BF16, EV, CH, STEP>(r, p, col, E);
+        load_param_as<SN_BF16, EV, CH>(r, p, col, step, E);
     } else {
-        load_param_as<SN_F16, EV, CH, STEP>(r, p, col, E);
+        load_param_as<SN_F16, EV, CH>(r, p, col, step, E);
     }
 }
 // lanes of one block of 32 are neighbours; every lane of the wave takes part (features beyond E are zeros)
-template <int EV, int CH, int STEP>
-__device__ __forceinline__ void store_checkpoint(void *codes, void *exps, int64_t row, int col, int npad, const Row<EV, CH> &r)
+template <int EV, int CH>
+__device__ __forceinline__ void store_checkpoint(void *codes, void *exps, int64_t row, int col, int step, int npad, const Row<EV, CH> &r)
 {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int j = col + c * STEP;
+        const int j = col + c * step;
         const uint32_t e = block_exp(block_top<EV>(r.v[c]));
         uint32_t q[EV / 4];
         encode<EV>(q, r.v[c], e);
@@ -202,8 +203,8 @@ __device__ __forceinline__ bool row_counts(const sn_block_norms_args &a, int64_t
 struct NormStats { float mean, rstd; };
 
 // mean and 1 / deviation of a row; elements beyond E do not count (they are zeros)
-template <int EV, int CH, int STEP, int WAVES>
-__device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, int E, bool tail, float inv_e, int rms, float eps, float *red, int &slot)
+template <int EV, int CH, bool MULTI>
+__device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, int step, int E, bool tail, float inv_e, int rms, float eps, float *red, int &slot)
 {
     NormStats s = {0.0f, 0.0f};
     if (!rms) {
@@ -212,7 +213,7 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < EV; ++i) t += r.v[c][i];
-        s.mean = row_sum<WAVES>(t, red, slot) * inv_e;
+        s.mean = row_sum<MULTI>(t, red, slot) * inv_e;
     }
     float q = 0.0f;
 #pragma unroll
@@ -220,29 +221,32 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
 #pragma unroll
         for (int i = 0; i < EV; ++i) {
             const float d = r.v[c][i] - s.mean;
-            q = !tail || col + c * STEP + i < E ? fmaf(d, d, q) : q;
+            q = !tail || col + c * step + i < E ? fmaf(d, d, q) : q;
         }
-    s.rstd = 1.0f / sqrtf(row_sum<WAVES>(q, red, slot) * inv_e + eps);
+    s.rstd = 1.0f / sqrtf(row_sum<MULTI>(q, red, slot) * inv_e + eps);
     return s;
 }
 
 // MODE: 0 = the parts of the call are looked up at run time; 1 = everything is there (2: but the gate), every row counts, nothing is
 // kept in 8 bits.  The branches of mode 0 make the compiler wait for all loads and stores in flight where it needs the oldest row,
 // the straight line of the others does not (rows of 4096 bf16, backward: 760 us for 32768 rows in mode 0, MODE_BWD_US in mode 1).
-template <int DT, int EV, int CH, int WAVES, int MODE>
-__global__ __launch_bounds__(block_of(WAVES)) void norms_forward_kernel(sn_block_norms_args a)
+template <int DT, int EV, int CH, bool MULTI, int MODE>
+__global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block_norms_args a)
 {
-    using L = Layout<DT, EV, CH, WAVES>;
-    constexpr int STEP = L::kStep;
+    using L = Layout<DT, EV, CH, MULTI>;
     constexpr bool ALL = MODE != 0;
-    __shared__ float red[32];
+    __shared__ __align__(16) float red[32];
+    if constexpr (MULTI) {
+        if (threadIdx.x < 32) red[threadIdx.x] = 0.0f;
+        __syncthreads();
+    }
     int slot = 0;
-    const int group = WAVES > 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
-    const int E = a.width, col = t * EV, npad = (E + 31) & ~31;
+    const int group = MULTI ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = MULTI ? threadIdx.x : threadIdx.x & 63;
+    const int E = a.width, step = (MULTI ? (int)blockDim.x : 64) * EV, col = t * EV, npad = (E + 31) & ~31;
     const float inv_e = 1.0f / (float)E;
     const bool gated = ALL ? MODE == 1 : a.gate != nullptr, post = ALL || a.has_post, pre = ALL || a.has_pre, keep = !ALL && a.x_codes;
-    const bool tail = __any(tail_shift<EV>(col + (CH - 1) * STEP, E) > 0);
+    const bool tail = __any(tail_shift<EV>(col + (CH - 1) * step, E) > 0);
     const int64_t turn = (int64_t)gridDim.x * L::kRows;
 
     struct Slot { Ahead<DT, EV, CH> x, f, z; bool live; };
@@ -252,40 +256,40 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_forward_kernel(sn_block
             s.live = row_counts(a, row);
             if (!s.live) return;
         }
-        issue_cols<DT, EV, CH, STEP, L::kTiny>(s.x, a.x, row, a.x_stride, col, E);
-        issue_cols<DT, EV, CH, STEP, L::kTiny>(s.f, a.branch, row, a.branch_stride, col, E);
-        if (gated) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.z, a.gate, row, a.gate_stride, col, E);
+        issue_cols<DT, EV, CH, L::kTiny>(s.x, a.x, row, a.x_stride, col, step, E);
+        issue_cols<DT, EV, CH, L::kTiny>(s.f, a.branch, row, a.branch_stride, col, step, E);
+        if (gated) issue_cols<DT, EV, CH, L::kTiny>(s.z, a.gate, row, a.gate_stride, col, step, E);
     };
     const int64_t start = (int64_t)blockIdx.x * L::kRows + group;
     Slot s0, s1;
     issue(s0, start);
-    if constexpr (L::kAhead == 2) issue(s1, start + turn);
+    if constexpr (L::kAheadForward == 2) issue(s1, start + turn);
     Row<EV, CH> w1, b1, sc, w2, b2;
-    load_param<EV, CH, STEP>(sc, a.scale, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(b1, post ? a.post_bias : nullptr, a.param_dtype, col, E, 0.0f);
-    load_param<EV, CH, STEP>(w2, pre ? a.pre_weight : nullptr, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(b2, pre ? a.pre_bias : nullptr, a.param_dtype, col, E, 0.0f);
+    load_param<EV, CH>(sc, a.scale, a.param_dtype, col, step, E, 1.0f);
+    load_param<EV, CH>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
+    load_param<EV, CH>(b1, post ? a.post_bias : nullptr, a.param_dtype, col, step, E, 0.0f);
+    load_param<EV, CH>(w2, pre ? a.pre_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
+    load_param<EV, CH>(b2, pre ? a.pre_bias : nullptr, a.param_dtype, col, step, E, 0.0f);
 
     auto work = [&](Slot &s, int64_t row) {
         if (!ALL && !s.live) {                               // the same for every wave of the row
-            issue(s, row + L::kAhead * turn);
-            zero_cols<DT, EV, CH, STEP>(a.y, row, col, E);
-            if (pre) zero_cols<DT, EV, CH, STEP>(a.h, row, col, E);
+            issue(s, row + L::kAheadForward * turn);
+            zero_cols<DT, EV, CH>(a.y, row, col, step, E);
+            if (pre) zero_cols<DT, EV, CH>(a.h, row, col, step, E);
             return;
         }
         Row<EV, CH> x, f, z;
-        take_cols<DT, EV, CH, STEP>(x, s.x, col, E, tail);
-        take_cols<DT, EV, CH, STEP>(f, s.f, col, E, tail);
-        if (gated) take_cols<DT, EV, CH, STEP>(z, s.z, col, E, tail);
-        issue(s, row + L::kAhead * turn);
+        take_cols<DT, EV, CH>(x, s.x, col, step, E, tail);
+        take_cols<DT, EV, CH>(f, s.f, col, step, E, tail);
+        if (gated) take_cols<DT, EV, CH>(z, s.z, col, step, E, tail);
+        issue(s, row + L::kAheadForward * turn);
         if (keep) {
-            store_checkpoint<EV, CH, STEP>(a.x_codes, a.x_exps, row, col, npad, x);
-            store_checkpoint<EV, CH, STEP>(a.branch_codes, a.branch_exps, row, col, npad, f);
-            if (gated) store_checkpoint<EV, CH, STEP>(a.gate_codes, a.gate_exps, row, col, npad, z);
+            store_checkpoint<EV, CH>(a.x_codes, a.x_exps, row, col, step, npad, x);
+            store_checkpoint<EV, CH>(a.branch_codes, a.branch_exps, row, col, step, npad, f);
+            if (gated) store_checkpoint<EV, CH>(a.gate_codes, a.gate_exps, row, col, step, npad, z);
         }
         NormStats n1 = {0.0f, 1.0f}, n2 = {0.0f, 1.0f};
-        if (post) n1 = statistics<EV, CH, STEP, WAVES>(f, col, E, tail, inv_e, a.rms, a.eps, red, slot);
+        if (post) n1 = statistics<EV, CH, MULTI>(f, col, step, E, tail, inv_e, a.rms, a.eps, red, slot);
         // (columns beyond E: inputs, weights and biases are zeros there, and so is y)
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -296,41 +300,44 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_forward_kernel(sn_block
                 if (gated) p *= sigmoid<DT>(z.v[c][i]);
                 x.v[c][i] = fmaf(p, sc.v[c][i], x.v[c][i]);
             }
-        store_cols<DT, EV, CH, STEP>(a.y, row, col, E, x);
+        store_cols<DT, EV, CH>(a.y, row, col, step, E, x);
         if (pre) {
-            n2 = statistics<EV, CH, STEP, WAVES>(x, col, E, tail, inv_e, a.rms, a.eps, red, slot);
+            n2 = statistics<EV, CH, MULTI>(x, col, step, E, tail, inv_e, a.rms, a.eps, red, slot);
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < EV; ++i) x.v[c][i] = fmaf((x.v[c][i] - n2.mean) * n2.rstd, w2.v[c][i], b2.v[c][i]);
-            store_cols<DT, EV, CH, STEP>(a.h, row, col, E, x);
+            store_cols<DT, EV, CH>(a.h, row, col, step, E, x);
         }
         if (a.stats && t == 0) *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(n1.mean, n1.rstd, n2.mean, n2.rstd);
     };
-    for (int64_t row = start; row < a.rows; row += L::kAhead * turn) {
+    for (int64_t row = start; row < a.rows; row += L::kAheadForward * turn) {
         work(s0, row);
-        if constexpr (L::kAhead == 2) {
+        if constexpr (L::kAheadForward == 2) {
             if (row + turn >= a.rows) break;
             work(s1, row + turn);
         }
     }
 }
 
-template <int DT, int EV, int CH, int WAVES, int MODE, bool KEPT>
-__global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_block_norms_args a, float *partial)
+template <int DT, int EV, int CH, bool MULTI, int MODE, bool KEPT>
+__global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_block_norms_args a, float *partial)
 {
-    using L = Layout<DT, EV, CH, WAVES>;
-    constexpr int STEP = L::kStep;
+    using L = Layout<DT, EV, CH, MULTI>;
     constexpr bool ALL = MODE != 0;
-    __shared__ float red[32];
+    __shared__ __align__(16) float red[32];
+    if constexpr (MULTI) {
+        if (threadIdx.x < 32) red[threadIdx.x] = 0.0f;
+        __syncthreads();
+    }
     int slot = 0;
-    const int group = WAVES > 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
-    const int E = a.width, col = t * EV, npad = (E + 31) & ~31;
+    const int group = MULTI ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = MULTI ? threadIdx.x : threadIdx.x & 63;
+    const int E = a.width, step = (MULTI ? (int)blockDim.x : 64) * EV, col = t * EV, npad = (E + 31) & ~31;
     const float inv_e = 1.0f / (float)E;
     const bool gated = ALL ? MODE == 1 : KEPT ? a.gate_codes != nullptr : a.gate != nullptr;
     const bool post = ALL || a.has_post, has_dy = ALL || a.dy, has_dh = ALL || a.dh;
-    const bool tail = __any(tail_shift<EV>(col + (CH - 1) * STEP, E) > 0);
+    const bool tail = __any(tail_shift<EV>(col + (CH - 1) * step, E) > 0);
     const int64_t turn = (int64_t)gridDim.x * L::kRows;
 
     struct Slot {
@@ -346,51 +353,51 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
             if (!s.live) return;
         }
         if constexpr (KEPT) {
-            issue_kept<EV, CH, STEP>(s.kx, a.x_codes, a.x_exps, row, col, npad);
-            issue_kept<EV, CH, STEP>(s.kf, a.branch_codes, a.branch_exps, row, col, npad);
-            if (gated) issue_kept<EV, CH, STEP>(s.kz, a.gate_codes, a.gate_exps, row, col, npad);
+            issue_kept<EV, CH>(s.kx, a.x_codes, a.x_exps, row, col, step, npad);
+            issue_kept<EV, CH>(s.kf, a.branch_codes, a.branch_exps, row, col, step, npad);
+            if (gated) issue_kept<EV, CH>(s.kz, a.gate_codes, a.gate_exps, row, col, step, npad);
         } else {
-            issue_cols<DT, EV, CH, STEP, L::kTiny>(s.x, a.x, row, a.x_stride, col, E);
-            issue_cols<DT, EV, CH, STEP, L::kTiny>(s.f, a.branch, row, a.branch_stride, col, E);
-            if (gated) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.z, a.gate, row, a.gate_stride, col, E);
+            issue_cols<DT, EV, CH, L::kTiny>(s.x, a.x, row, a.x_stride, col, step, E);
+            issue_cols<DT, EV, CH, L::kTiny>(s.f, a.branch, row, a.branch_stride, col, step, E);
+            if (gated) issue_cols<DT, EV, CH, L::kTiny>(s.z, a.gate, row, a.gate_stride, col, step, E);
         }
-        if (has_dy) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.dy, a.dy, row, a.dy_stride, col, E);
-        if (has_dh) issue_cols<DT, EV, CH, STEP, L::kTiny>(s.dh, a.dh, row, a.dh_stride, col, E);
+        if (has_dy) issue_cols<DT, EV, CH, L::kTiny>(s.dy, a.dy, row, a.dy_stride, col, step, E);
+        if (has_dh) issue_cols<DT, EV, CH, L::kTiny>(s.dh, a.dh, row, a.dh_stride, col, step, E);
         s.st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
     };
     const int64_t start = (int64_t)blockIdx.x * L::kRows + group;
     Slot s0, s1;
     issue(s0, start);
-    if constexpr (L::kAhead == 2) issue(s1, start + turn);
+    if constexpr (L::kAheadBackward == 2) issue(s1, start + turn);
     Row<EV, CH> w1, b1, sc, w2;
-    load_param<EV, CH, STEP>(sc, a.scale, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, E, 1.0f);
-    load_param<EV, CH, STEP>(b1, post ? a.post_bias : nullptr, a.param_dtype, col, E, 0.0f);
-    load_param<EV, CH, STEP>(w2, has_dh ? a.pre_weight : nullptr, a.param_dtype, col, E, 1.0f);
+    load_param<EV, CH>(sc, a.scale, a.param_dtype, col, step, E, 1.0f);
+    load_param<EV, CH>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
+    load_param<EV, CH>(b1, post ? a.post_bias : nullptr, a.param_dtype, col, step, E, 0.0f);
+    load_param<EV, CH>(w2, has_dh ? a.pre_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
     Row<EV, CH> sum[kVectors] = {};
 
     auto work = [&](Slot &s, int64_t row) {
         if (!ALL && !s.live) {
-            issue(s, row + L::kAhead * turn);
-            if (a.dx) zero_cols<DT, EV, CH, STEP>(a.dx, row, col, E);
-            if (a.dbranch) zero_cols<DT, EV, CH, STEP>(a.dbranch, row, col, E);
-            if (a.dgate) zero_cols<DT, EV, CH, STEP>(a.dgate, row, col, E);
+            issue(s, row + L::kAheadBackward * turn);
+            if (a.dx) zero_cols<DT, EV, CH>(a.dx, row, col, step, E);
+            if (a.dbranch) zero_cols<DT, EV, CH>(a.dbranch, row, col, step, E);
+            if (a.dgate) zero_cols<DT, EV, CH>(a.dgate, row, col, step, E);
             return;
         }
         Row<EV, CH> x, f, z, u = {}, d;
         if constexpr (KEPT) {
-            take_kept<EV, CH, STEP>(x, s.kx, col, npad);
-            take_kept<EV, CH, STEP>(f, s.kf, col, npad);
-            if (gated) take_kept<EV, CH, STEP>(z, s.kz, col, npad);
+            take_kept<EV, CH>(x, s.kx, col, step, npad);
+            take_kept<EV, CH>(f, s.kf, col, step, npad);
+            if (gated) take_kept<EV, CH>(z, s.kz, col, step, npad);
         } else {
-            take_cols<DT, EV, CH, STEP>(x, s.x, col, E, tail);
-            take_cols<DT, EV, CH, STEP>(f, s.f, col, E, tail);
-            if (gated) take_cols<DT, EV, CH, STEP>(z, s.z, col, E, tail);
+            take_cols<DT, EV, CH>(x, s.x, col, step, E, tail);
+            take_cols<DT, EV, CH>(f, s.f, col, step, E, tail);
+            if (gated) take_cols<DT, EV, CH>(z, s.z, col, step, E, tail);
         }
-        if (has_dy) take_cols<DT, EV, CH, STEP>(u, s.dy, col, E, tail);
-        if (has_dh) take_cols<DT, EV, CH, STEP>(d, s.dh, col, E, tail);
+        if (has_dy) take_cols<DT, EV, CH>(u, s.dy, col, step, E, tail);
+        if (has_dh) take_cols<DT, EV, CH>(d, s.dh, col, step, E, tail);
         const float4 st = s.st;
-        issue(s, row + L::kAhead * turn);
+        issue(s, row + L::kAheadBackward * turn);
         // f -> unit values of the post norm, z -> sigmoid, x -> unit values of y.  Columns beyond E hold whatever the statistics make of
         // zeros: every use multiplies it by a weight or a gradient that is zero there, and no store takes it.
 #pragma unroll
@@ -417,7 +424,7 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
                     m1 += d.v[c][i];
                     m2 = fmaf(d.v[c][i], x.v[c][i], m2);
                 }
-            row_sum2<WAVES>(m1, m2, red, slot);
+            row_sum2<MULTI>(m1, m2, red, slot);
             m1 = a.rms ? 0.0f : m1 * inv_e;
             m2 *= inv_e;
 #pragma unroll
@@ -425,7 +432,7 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
 #pragma unroll
                 for (int i = 0; i < EV; ++i) u.v[c][i] = fmaf(st.w, fmaf(-x.v[c][i], m2, d.v[c][i] - m1), u.v[c][i]);
         }
-        if (ALL || a.dx) store_cols<DT, EV, CH, STEP>(a.dx, row, col, E, u);
+        if (ALL || a.dx) store_cols<DT, EV, CH>(a.dx, row, col, step, E, u);
         // d -> gradient of the gated product's p, x -> gradient of the gate
         float m1 = 0.0f, m2 = 0.0f;
 #pragma unroll
@@ -443,9 +450,9 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
                 m1 += d.v[c][i];
                 m2 = fmaf(d.v[c][i], f.v[c][i], m2);
             }
-        if (gated && (ALL || a.dgate)) store_cols<DT, EV, CH, STEP>(a.dgate, row, col, E, x);
+        if (gated && (ALL || a.dgate)) store_cols<DT, EV, CH>(a.dgate, row, col, step, E, x);
         if (post) {
-            row_sum2<WAVES>(m1, m2, red, slot);
+            row_sum2<MULTI>(m1, m2, red, slot);
             m1 = a.rms ? 0.0f : m1 * inv_e;
             m2 *= inv_e;
 #pragma unroll
@@ -453,11 +460,11 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
 #pragma unroll
                 for (int i = 0; i < EV; ++i) d.v[c][i] = st.y * fmaf(-f.v[c][i], m2, d.v[c][i] - m1);
         }
-        if (ALL || a.dbranch) store_cols<DT, EV, CH, STEP>(a.dbranch, row, col, E, d);
+        if (ALL || a.dbranch) store_cols<DT, EV, CH>(a.dbranch, row, col, step, E, d);
     };
-    for (int64_t row = start; row < a.rows; row += L::kAhead * turn) {
+    for (int64_t row = start; row < a.rows; row += L::kAheadBackward * turn) {
         work(s0, row);
-        if constexpr (L::kAhead == 2) {
+        if constexpr (L::kAheadBackward == 2) {
             if (row + turn >= a.rows) break;
             work(s1, row + turn);
         }
@@ -465,20 +472,20 @@ __global__ __launch_bounds__(block_of(WAVES)) void norms_backward_kernel(sn_bloc
     if (partial) {
         // the workgroup's rows side by side are added here, one line of partial sums leaves for each workgroup
         float *dst = partial + (int64_t)blockIdx.x * kVectors * E;
-        __shared__ float join[L::kRows > 1 ? L::kRows * L::kWidth : 1];
+        __shared__ float join[MULTI ? 1 : L::kRows * L::kWidth];
 #pragma unroll
         for (int k = 0; k < kVectors; ++k) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < EV; ++i) {
-                    const int j = col + c * STEP + i;
-                    if constexpr (L::kRows > 1) join[group * L::kWidth + j] = sum[k].v[c][i];
+                    const int j = col + c * step + i;
+                    if constexpr (!MULTI) join[group * L::kWidth + j] = sum[k].v[c][i];
                     else if (j < E) dst[(int64_t)k * E + j] = sum[k].v[c][i];
                 }
-            if constexpr (L::kRows > 1) {
+            if constexpr (!MULTI) {
                 __syncthreads();
-                for (int j = threadIdx.x; j < E; j += L::kBlock) {
+                for (int j = threadIdx.x; j < E; j += 256) {
                     float v = join[j];
 #pragma unroll
                     for (int g = 1; g < L::kRows; ++g) v += join[g * L::kWidth + j];
@@ -514,18 +521,13 @@ __global__ __launch_bounds__(1024) void norms_columns_kernel(const float *partia
 }
 
 // lanes of a row: 8 elements a lane up to 4096 columns (16 waves with five column sums each would spill); 4 a lane under 257 columns
-int waves_for(int E)
-{
-    int w = 1;
-    while (w * 512 < E) w *= 2;
-    return w;
-}
+int waves_for(int E) { return (E + 511) / 512; }
 int rows_per_block(int E) { return waves_for(E) > 1 ? 1 : 4; }
 int backward_blocks(int64_t rows, int E)
 {
     const int64_t turns = (rows + rows_per_block(E) - 1) / rows_per_block(E);
     // as many workgroups as are resident with the registers of the backward kernel: two waves a SIMD (one wave a row of up to 256: four)
-    const int64_t most = waves_for(E) == 1 ? 1024 : 2048 / waves_for(E), each = (turns + most - 1) / most;
+    const int64_t most = waves_for(E) == 1 ? 1024 : 256 * (8 / waves_for(E)), each = (turns + most - 1) / most;
     return (int)((turns + each - 1) / each);                 // (the same number of turns for all but the last)
 }
 
@@ -542,19 +544,18 @@ int check_args(const sn_block_norms_args *a, const char *who)
     return SN_OK;
 }
 
-template <int DT, int EV, int CH, int WAVES> int launch_forward(const sn_block_norms_args &a, hipStream_t st)
+template <int DT, int EV, int CH, bool MULTI> int launch_forward(const sn_block_norms_args &a, hipStream_t st)
 {
-    using L = Layout<DT, EV, CH, WAVES>;
-    const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = WAVES == 1 ? 2048 : 4096 / WAVES, each = (turns + most - 1) / most;
+    using L = Layout<DT, EV, CH, MULTI>;
+    const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = MULTI ? 256 * (16 / waves_for(a.width)) : 2048, each = (turns + most - 1) / most;
     const bool all = a.has_post && a.has_pre && !a.n_valid && !a.x_codes;
-    const auto kernel = !all ? norms_forward_kernel<DT, EV, CH, WAVES, 0> : a.gate ? norms_forward_kernel<DT, EV, CH, WAVES, 1> : norms_forward_kernel<DT, EV, CH, WAVES, 2>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((turns + each - 1) / each)), dim3(L::kBlock), 0, st, a);
+    const auto kernel = !all ? norms_forward_kernel<DT, EV, CH, MULTI, 0> : a.gate ? norms_forward_kernel<DT, EV, CH, MULTI, 1> : norms_forward_kernel<DT, EV, CH, MULTI, 2>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((turns + each - 1) / each)), dim3(MULTI ? waves_for(a.width) * 64 : 256), 0, st, a);
     SN_CHECK_LAUNCH("sn_block_norms_forward");
     return SN_OK;
 }
-template <int DT, int EV, int CH, int WAVES> int launch_backward(const sn_block_norms_args &a, hipStream_t st)
+template <int DT, int EV, int CH, bool MULTI> int launch_backward(const sn_block_norms_args &a, hipStream_t st)
 {
-    using L = Layout<DT, EV, CH, WAVES>;
     const int blocks = backward_blocks(a.rows, a.width);
     const ColumnOut out = {{a.dpre_weight, a.dpre_bias, a.dscale, a.dpost_weight, a.dpost_bias}};
     bool columns = false;
@@ -562,11 +563,11 @@ template <int DT, int EV, int CH, int WAVES> int launch_backward(const sn_block_
     float *partial = columns ? (float *)a.workspace : nullptr;
     const bool gate = a.x_codes ? a.gate_codes != nullptr : a.gate != nullptr;
     const bool all = a.has_post && a.has_pre && !a.n_valid && a.dy && a.dh && a.dx && a.dbranch && (!gate || a.dgate);
-    const auto kernel = a.x_codes ? (!all ? norms_backward_kernel<DT, EV, CH, WAVES, 0, true> : gate ? norms_backward_kernel<DT, EV, CH, WAVES, 1, true>
-                                                                                                      : norms_backward_kernel<DT, EV, CH, WAVES, 2, true>)
-                                  : (!all ? norms_backward_kernel<DT, EV, CH, WAVES, 0, false> : gate ? norms_backward_kernel<DT, EV, CH, WAVES, 1, false>
-                                                                                                       : norms_backward_kernel<DT, EV, CH, WAVES, 2, false>);
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(L::kBlock), 0, st, a, partial);
+    const auto kernel = a.x_codes ? (!all ? norms_backward_kernel<DT, EV, CH, MULTI, 0, true> : gate ? norms_backward_kernel<DT, EV, CH, MULTI, 1, true>
+                                                                                                      : norms_backward_kernel<DT, EV, CH, MULTI, 2, true>)
+                                  : (!all ? norms_backward_kernel<DT, EV, CH, MULTI, 0, false> : gate ? norms_backward_kernel<DT, EV, CH, MULTI, 1, false>
+                                                                                                       : norms_backward_kernel<DT, EV, CH, MULTI, 2, false>);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(MULTI ? waves_for(a.width) * 64 : 256), 0, st, a, partial);
     SN_CHECK_LAUNCH("sn_block_norms_backward");
     if (columns) {
         hipLaunchKernelGGL(norms_columns_kernel, dim3((a.width + 31) / 32, kVectors), dim3(1024), 0, st, partial, blocks, a.width, out, a.param_dtype);
@@ -577,18 +578,14 @@ template <int DT, int EV, int CH, int WAVES> int launch_backward(const sn_block_
 
 template <bool FORWARD, int DT, int EV, int CH> int by_waves(const sn_block_norms_args &a, hipStream_t st)
 {
-    switch (waves_for(a.width)) {
-#define SN_CASE(W) case W: if constexpr (FORWARD) return launch_forward<DT, EV, CH, W>(a, st); else return launch_backward<DT, EV, CH, W>(a, st);
-        SN_CASE(1) SN_CASE(2) SN_CASE(4)
-#undef SN_CASE
-        default: if constexpr (FORWARD) return launch_forward<DT, EV, CH, 8>(a, st); else return launch_backward<DT, EV, CH, 8>(a, st);
-    }
+    if constexpr (FORWARD) return waves_for(a.width) > 1 ? launch_forward<DT, EV, CH, true>(a, st) : launch_forward<DT, EV, CH, false>(a, st);
+    else return waves_for(a.width) > 1 ? launch_backward<DT, EV, CH, true>(a, st) : launch_backward<DT, EV, CH, false>(a, st);
 }
 template <bool FORWARD, int DT> int by_width(const sn_block_norms_args &a, hipStream_t st)
 {
     if (a.width <= 256) {
-        if constexpr (FORWARD) return launch_forward<DT, 4, 1, 1>(a, st);
-        else return launch_backward<DT, 4, 1, 1>(a, st);
+        if constexpr (FORWARD) return launch_forward<DT, 4, 1, false>(a, st);
+        else return launch_backward<DT, 4, 1, false>(a, st);
     }
     if constexpr (DT == SN_F32) return by_waves<FORWARD, DT, 4, 2>(a, st);
     else return by_waves<FORWARD, DT, 8, 1>(a, st);

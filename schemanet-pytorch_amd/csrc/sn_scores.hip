@@ -5,10 +5,11 @@
 // them), backward reads them once and writes the gradient.  A row belongs to one wave (up to kWaveRow entries), to the four
 // waves of a workgroup, or - few rows - to up to 64 workgroups whose partial results a second launch joins.
 //
-// Top list: a wave keeps its k best (value, index) sorted across its lanes, lane j the j-th.  A group of elements is looked at
-// again only if one of them beats the k-th; an insertion is one ballot (its place) and one shift by a lane.  Order: larger value
-// first, lower index among equals.  Lists are joined in pairs: an element's place in the join is its own plus the number of
-// the partner's that come before it (binary search).
+// Top list: a wave keeps its k best (value, index) sorted across its lanes, lane j the j-th.  The first 1024 elements fill it through a
+// bound that the lanes' maxima give (fill_list); after that a group of elements is looked at again only if one of them beats
+// the k-th, and an insertion is one ballot (its place) and one shift by a lane.  Order: larger value first, lower index among
+// equals.  Lists are joined in pairs: an element's place in the join is its own plus the number of the partner's that come
+// before it (binary search).
 #include "sn_typed.h"
 
 namespace {
@@ -21,7 +22,7 @@ constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 // stands for any distance beyond it where it is multiplied by exp(d): exp(-10^4) = 0 in fp32, and 0 times an infinite d must stay 0
 constexpr float kFar = -1.0e4f;
-constexpr int kNone = 0x7FFFFFFF;
+constexpr float kLowest = -3.402823466e38f;
 
 struct Soft { float m, s, t; };
 
@@ -53,62 +54,153 @@ __device__ __forceinline__ Soft wave_join(Soft a)
     return a;
 }
 
-__device__ __forceinline__ bool before(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
+// An entry as one number that orders like (value, then the lower index): the value's bits turned so that they order as an unsigned
+// number, over the index's complement.  -0 counts as 0.  kNone: an entry that was never filled; no logit at -inf enters a list.
+typedef uint64_t Key;
+constexpr Key kNone = 0x007FFFFF00000000ull;                 // (-inf, -1)
+__device__ __forceinline__ Key key_of(float v, int i)
+{
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return ((Key)(b ^ ((uint32_t)((int)b >> 31) | 0x80000000u)) << 32) | (uint32_t)~i;
+}
+__device__ __forceinline__ float key_value(Key k)
+{
+    const uint32_t b = (uint32_t)(k >> 32);
+    return __uint_as_float(b ^ ((uint32_t)((int)~b >> 31) | 0x80000000u));
+}
+__device__ __forceinline__ int key_index(Key k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ Key lane_key(Key k, int lane)
+{
+    return ((Key)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+}
+
+// value of lane ^ STRIDE without LDS: quad permutations, mirrors and rotations of 16 lanes, swaps of 16 and 32
+template <int STRIDE> __device__ __forceinline__ uint32_t lane_xor(uint32_t v)
+{
+    if constexpr (STRIDE == 1) return SN_DPP_U32(v, 0xB1);
+    else if constexpr (STRIDE == 2) return SN_DPP_U32(v, 0x4E);
+    else if constexpr (STRIDE == 4) return SN_DPP_U32(SN_DPP_U32(v, 0x1B), 0x141);      // 3 - i in the quad, then 7 - i in the half row
+    else if constexpr (STRIDE == 8) return SN_DPP_U32(v, 0x128);                        // row_ror:8
+    else if constexpr (STRIDE == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & 32) ? r[0] : r[1];
+    }
+}
+__device__ __forceinline__ float other_lane(float v, float o, bool first) { return first ? fmaxf(v, o) : fminf(v, o); }
+__device__ __forceinline__ Key other_lane(Key v, Key o, bool first) { return (o > v) == first ? o : v; }
+template <int STRIDE> __device__ __forceinline__ float lane_xor(float v) { return __uint_as_float(lane_xor<STRIDE>(__float_as_uint(v))); }
+template <int STRIDE> __device__ __forceinline__ Key lane_xor(Key v)
+{
+    return ((Key)lane_xor<STRIDE>((uint32_t)(v >> 32)) << 32) | lane_xor<STRIDE>((uint32_t)v);
+}
+template <int SIZE, int STRIDE, class T> __device__ __forceinline__ void sort_merge(T &v, int lane)
+{
+    // the lower lane of a pair keeps the larger one in the blocks that are sorted downwards
+    const bool first = ((lane & STRIDE) == 0) == ((lane & SIZE) == 0 || SIZE == 64);
+    v = other_lane(v, lane_xor<STRIDE>(v), first);
+    if constexpr (STRIDE > 1) sort_merge<SIZE, STRIDE / 2>(v, lane);
+}
+// the wave's 64 numbers (no NaN) in order, lane 0 the largest: bitonic
+template <class T> __device__ __forceinline__ void wave_sort(T &v)
+{
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));           // (the 21 lane masks are made here, not kept in scalar registers over the caller's loop)
+    sort_merge<2, 1>(v, lane);
+    sort_merge<4, 2>(v, lane);
+    sort_merge<8, 4>(v, lane);
+    sort_merge<16, 8>(v, lane);
+    sort_merge<32, 16>(v, lane);
+    sort_merge<64, 32>(v, lane);
+}
 
 // sorted list of a wave
 struct TopList {
-    float v;
-    int i;
-    float last_v;         // the k-th entry, in every lane
-    int last_i;
-    __device__ __forceinline__ void reset() { v = -INFINITY; i = kNone; last_v = -INFINITY; last_i = kNone; }
-    // (nv, ni): the same in every lane, before the k-th entry
-    __device__ __forceinline__ void insert(float nv, int ni, int k)
+    Key key, last;        // this lane's entry; the k-th entry, in every lane
+    float last_v;
+    __device__ __forceinline__ void reset() { key = last = kNone; last_v = -INFINITY; }
+    __device__ __forceinline__ void set_last(int k)
+    {
+        last = lane_key(key, k - 1);
+        last_v = key_value(last);
+    }
+    // n: the same in every lane, before the k-th entry
+    __device__ __forceinline__ void insert(Key n, int k)
     {
         const int lane = threadIdx.x & 63;
-        const int pos = __popcll(__ballot(before(v, i, nv, ni)));
-        const float up_v = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x138, 0xF, 0xF, false));     // wave_shr:1
-        const int up_i = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xF, 0xF, false);
-        v = lane > pos ? up_v : lane == pos ? nv : v;
-        i = lane > pos ? up_i : lane == pos ? ni : i;
-        last_v = SN_READLANE_F32(v, k - 1);
-        last_i = __builtin_amdgcn_readlane(i, k - 1);
+        const int pos = __popcll(__ballot(key > n));
+        const uint32_t up_hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(key >> 32), 0x138, 0xF, 0xF, false);        // wave_shr:1
+        const uint32_t up_lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)key, 0x138, 0xF, 0xF, false);
+        key = lane > pos ? ((Key)up_hi << 32) | up_lo : lane == pos ? n : key;
+        set_last(k);
     }
-    __device__ __forceinline__ void offer(float x, int ix, int k)
+    __device__ __forceinline__ void offer(float x, int i, int k)
     {
-        uint64_t b = __ballot(before(x, ix, last_v, last_i));
+        const Key mine = key_of(x, i);
+        uint64_t b = __ballot(x >= last_v && mine > last && x > -INFINITY);      // (NaN: not)
         while (b) {
             const int l = __builtin_ctzll(b);
-            const float nv = SN_READLANE_F32(x, l);
-            const int ni = __builtin_amdgcn_readlane(ix, l);
-            insert(nv, ni, k);
-            b = __ballot(before(x, ix, last_v, last_i) && (threadIdx.x & 63) > l);
+            insert(lane_key(mine, l), k);
+            b &= b - 1;
+            b &= __ballot(mine > last);
         }
     }
 };
 
+// Fill an empty list from N elements a lane (x, their indexes index(u)): the k-th largest of the 64 lanes' maxima is a bound that at
+// least k elements reach; those that do are gathered and sorted.  -> false (nothing done) if more than 64 do.  room: 64 entries of
+// LDS of this wave
+template <int N, class Index> __device__ __forceinline__ bool fill_list(TopList &top, const float (&x)[N], float lane_max, Index index, int k, Key *room)
+{
+    const int lane = threadIdx.x & 63;
+    float b = lane_max;
+    wave_sort(b);
+    const float bound = fmaxf(SN_READLANE_F32(b, k - 1), kLowest);               // (never an entry at -inf)
+    int count = 0, at[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const uint64_t m = __ballot(x[u] >= bound);
+        at[u] = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        count += __popcll(m);
+    }
+    if (count > 64) return false;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+        if (x[u] >= bound) room[at[u]] = key_of(x[u], index(u));
+    __builtin_amdgcn_wave_barrier();                         // (one wave's LDS operations stay in order)
+    top.key = lane < count ? room[lane] : kNone;
+    wave_sort(top.key);
+    if (lane >= k) top.key = kNone;
+    top.set_last(k);
+    return true;
+}
+
 // the wave's share (segments w, w + nw, ...) of entries c0 .. c1 - 1 of a row
 template <int DT, bool TOP>
-__device__ __forceinline__ void scan(const void *row, int64_t c0, int64_t c1, int w, int nw, Soft &soft, TopList &top, int k)
+__device__ __forceinline__ void scan(const void *row, int64_t c0, int64_t c1, int w, int nw, Soft &soft, TopList &top, int k, Key *room)
 {
-    constexpr int EV = DT == SN_F32 ? 4 : 8, PER = 2, SEG = 64 * EV * PER;
+    constexpr int EV = DT == SN_F32 ? 4 : 8, PER = 16 / EV, SEG = 64 * 16;
     const int lane = threadIdx.x & 63;
     const char *base = (const char *)row + c0 * (DT == SN_F32 ? 4 : 2);
     const int n = (int)(c1 - c0);
     const uint32_t fill = DT == SN_F32 ? 0xFF800000u : DT == SN_BF16 ? 0xFF80u : 0xFC00u;      // -inf
+    bool empty = true;
     for (int s0 = w * SEG; s0 < n; s0 += nw * SEG) {
-        float x[PER][EV];
+        float x[16];
 #pragma unroll
         for (int c = 0; c < PER; ++c) {
             uint32_t raw[words<DT, EV>()];
             load_raw<DT, EV>(raw, base, s0 + (c * 64 + lane) * EV, n, fill);
-            unpack<DT, EV>(x[c], raw);
+            float part[EV];
+            unpack<DT, EV>(part, raw);
+#pragma unroll
+            for (int e = 0; e < EV; ++e) x[c * EV + e] = part[e];
         }
-        float m = x[0][0];
+        float m = x[0];
 #pragma unroll
-        for (int c = 0; c < PER; ++c)
-#pragma unroll
-            for (int e = 0; e < EV; ++e) m = fmaxf(m, x[c][e]);
+        for (int u = 1; u < 16; ++u) m = fmaxf(m, x[u]);
         const float mx = fmaxf(m, soft.m);
         if (mx > soft.m) {
             const float d = soft.m - mx, f = exp_fast(d);
@@ -118,22 +210,20 @@ __device__ __forceinline__ void scan(const void *row, int64_t c0, int64_t c1, in
         }
         const float ref = soft.m == -INFINITY ? 0.0f : soft.m;
 #pragma unroll
-        for (int c = 0; c < PER; ++c)
-#pragma unroll
-            for (int e = 0; e < EV; ++e) {
-                const float d = x[c][e] - ref, p = exp_fast(d);
-                soft.s += p;
-                soft.t = fmaf(p, fmaxf(d, kFar), soft.t);
-            }
+        for (int u = 0; u < 16; ++u) {
+            const float d = x[u] - ref, p = exp_fast(d);
+            soft.s += p;
+            soft.t = fmaf(p, fmaxf(d, kFar), soft.t);
+        }
         if constexpr (TOP) {
-            if (__any(m > top.last_v) || top.last_i == kNone) {
+            auto index = [&](int u) { return (int)c0 + s0 + ((u / EV) * 64 + lane) * EV + u % EV; };
+            if (__any(m > top.last_v)) {
+                // (m is NaN only where every element of the lane is: none of them is a candidate)
+                if (!empty || !fill_list(top, x, m == m ? m : -INFINITY, index, k, room)) {
 #pragma unroll
-                for (int c = 0; c < PER; ++c)
-#pragma unroll
-                    for (int e = 0; e < EV; ++e) {
-                        const int j = s0 + (c * 64 + lane) * EV + e;
-                        top.offer(j < n ? x[c][e] : -INFINITY, j < n ? (int)c0 + j : kNone, k);
-                    }
+                    for (int u = 0; u < 16; ++u) top.offer(x[u], index(u), k);
+                }
+                empty = false;
             }
         }
     }
@@ -148,7 +238,7 @@ struct ScoreArgs {
     int64_t per_split;
     float *log_probs, *entropy, *stats, *top_lp;
     int64_t *top_ids;
-    float *part;          // [rows, splits, 3 + 2 k]: m, s, t, values, indexes
+    float *part;          // [rows, splits, 4 + 2 k]: m, s, t, nothing, keys
 };
 
 template <int DT> __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, Soft s)
@@ -163,43 +253,65 @@ template <int DT> __device__ __forceinline__ void write_row(const ScoreArgs &a, 
     }
     a.log_probs[row] = lp;
     a.entropy[row] = h;
-    a.stats[row * 3] = s.m;
-    a.stats[row * 3 + 1] = s.s;
-    a.stats[row * 3 + 2] = h;
+    if (a.stats) {
+        a.stats[row * 3] = s.m;
+        a.stats[row * 3 + 1] = s.s;
+        a.stats[row * 3 + 2] = h;
+    }
 }
-__device__ __forceinline__ void write_top(const ScoreArgs &a, int64_t row, int j, float v, int i, Soft s)
+// the row's list, entry j by lane j of one wave (every lane of it calls; lanes from k on: kNone).  A row without NaN that has fewer than k
+// entries above -inf: the rest are its entries at -inf, the lowest index first - nearly all others are, so the first few hundred
+// hold enough.
+template <int DT> __device__ __forceinline__ void write_top(const ScoreArgs &a, int64_t row, Key key, Soft s)
 {
+    const int lane = threadIdx.x & 63;
     const float ls = logf(s.s);
-    a.top_lp[row * a.k + j] = s.s == 0.0f ? -INFINITY : i == kNone ? __uint_as_float(0x7FC00000u) : (v - s.m) - ls;
-    a.top_ids[row * a.k + j] = i == kNone ? -1 : i;
+    const bool nan = s.s != s.s;
+    float v = key_value(key);
+    int i = key_index(key);
+    int have = __popcll(__ballot(lane < a.k && key != kNone));
+    if (have < a.k && !nan) {
+        const void *p = (const char *)a.logits + row * a.stride * (DT == SN_F32 ? 4 : 2);
+        for (int64_t j0 = 0; have < a.k && j0 < a.n; j0 += 64) {
+            const bool masked = j0 + lane < a.n && load_one<DT>(p, j0 + lane) == -INFINITY;
+            const uint64_t m = __ballot(masked);
+            const int want = lane - have;                    // this lane takes the want-th of them
+            int seen = 0;
+            for (uint64_t r = m; r && seen < a.k - have; r &= r - 1, ++seen)
+                if (seen == want) i = (int)j0 + __builtin_ctzll(r);
+            have += __popcll(m);
+        }
+    }
+    if (lane < a.k) {
+        a.top_lp[row * a.k + lane] = nan ? __uint_as_float(0x7FC00000u) : v == -INFINITY ? -INFINITY : (v - s.m) - ls;
+        a.top_ids[row * a.k + lane] = i;
+    }
 }
 
-// `lists` sorted lists of k in src -> one, in pairs; both buffers hold lists * k entries.  Every thread of the workgroup calls.
-// -> the buffer that holds the result
-struct Entry { float v; int i; };
-__device__ Entry *join_lists(Entry *src, Entry *dst, int lists, int k)
+// `lists` sorted lists of k in src -> one, in pairs: an entry's place in the join is its own plus the number of the partner's that
+// come before it.  Both buffers hold lists * k entries.  Every thread of the workgroup calls.  -> the buffer that holds the result
+__device__ __forceinline__ Key *join_lists(Key *src, Key *dst, int lists, int k)
 {
     while (lists > 1) {
         const int total = lists * k;
         for (int e = threadIdx.x; e < total; e += blockDim.x) {
             const int l = e / k, j = e - l * k;
-            const Entry me = src[e];
+            const Key me = src[e];
             int pos = j;
             if ((l ^ 1) < lists) {
-                const Entry *o = src + (l ^ 1) * k;
-                int lo = 0, hi = k;                          // how many of the partner's come before this one
+                const Key *o = src + (l ^ 1) * k;
+                int lo = 0, hi = k;
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
-                    // (entries that were never filled are equal: those of the lower list first)
-                    const bool b = before(o[mid].v, o[mid].i, me.v, me.i) || (o[mid].v == me.v && o[mid].i == me.i && (l & 1));
-                    if (b) lo = mid + 1; else hi = mid;
+                    // (only entries that were never filled are equal: those of the lower list first)
+                    if (o[mid] > me || (o[mid] == me && (l & 1))) lo = mid + 1; else hi = mid;
                 }
                 pos += lo;
             }
             if (pos < k) dst[(l >> 1) * k + pos] = me;
         }
         __syncthreads();
-        Entry *const swap = src;
+        Key *const swap = src;
         src = dst;
         dst = swap;
         lists = (lists + 1) >> 1;
@@ -207,20 +319,66 @@ __device__ Entry *join_lists(Entry *src, Entry *dst, int lists, int k)
     return src;
 }
 
+// The k best of `lists` (at most 64) sorted lists of k in src, lane j of wave 0 the j-th: with j = ceil(k / lists), the ceil(k / j)-th
+// largest of the lists' j-th entries is a bound that k entries reach; those that do, if they are at most 64, are sorted by one wave,
+// otherwise the lists are joined in pairs.  Every thread of the workgroup calls, after a barrier behind the writing of src.
+struct Select { float bound; int counts[kScoreWaves]; Key room[64]; };
+__device__ __forceinline__ Key best_of_lists(Key *src, Key *other, int lists, int k, Select &sh)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, total = lists * k;
+    const int j = (k + lists - 1) / lists;
+    // (every wave finds the bound: no barrier for it)
+    float b = lane < lists ? key_value(src[lane * k + j - 1]) : -INFINITY;
+    wave_sort(b);
+    b = __shfl(b, (k + j - 1) / j - 1, 64);
+    int count = 0;
+    for (int e = threadIdx.x; e < total; e += kScoreThreads) {
+        const Key q = src[e];
+        count += q != kNone && key_value(q) >= b;
+    }
+    int upto = count;                                        // exclusive sum over the workgroup
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(upto, off, 64);
+        upto += lane >= off ? o : 0;
+    }
+    if (lane == 63) sh.counts[wave] = upto;
+    __syncthreads();
+    int all = 0, place = upto - count;
+#pragma unroll
+    for (int w = 0; w < kScoreWaves; ++w) {
+        place += w < wave ? sh.counts[w] : 0;
+        all += sh.counts[w];
+    }
+    if (all > 64) {
+        const Key *best = join_lists(src, other, lists, k);
+        return lane < k ? best[lane] : kNone;
+    }
+    for (int e = threadIdx.x; e < total; e += kScoreThreads) {
+        const Key q = src[e];
+        if (q != kNone && key_value(q) >= b) sh.room[place++] = q;
+    }
+    __syncthreads();
+    Key mine = lane < all ? sh.room[lane] : kNone;
+    if (wave == 0) wave_sort(mine);
+    return lane < k ? mine : kNone;
+}
+
 // one wave a row
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kScoreThreads) void scores_wave_kernel(ScoreArgs a)
 {
+    __shared__ Key room[TOP ? kScoreWaves : 1][TOP ? 64 : 1];
     const int lane = threadIdx.x & 63;
     const int64_t turn = (int64_t)gridDim.x * kScoreWaves;
     for (int64_t row = (int64_t)blockIdx.x * kScoreWaves + (threadIdx.x >> 6); row < a.rows; row += turn) {
         Soft soft = {-INFINITY, 0.0f, 0.0f};
         TopList top;
         top.reset();
-        scan<DT, TOP>((const char *)a.logits + row * a.stride * (DT == SN_F32 ? 4 : 2), 0, a.n, 0, 1, soft, top, a.k);
+        scan<DT, TOP>((const char *)a.logits + row * a.stride * (DT == SN_F32 ? 4 : 2), 0, a.n, 0, 1, soft, top, a.k, room[TOP ? threadIdx.x >> 6 : 0]);
         soft = wave_join(soft);
         if (lane == 0) write_row<DT>(a, row, soft);
-        if (TOP && lane < a.k) write_top(a, row, lane, top.v, top.i, soft);
+        if constexpr (TOP) write_top<DT>(a, row, top.key, soft);
     }
 }
 
@@ -229,7 +387,8 @@ template <int DT, bool TOP>
 __global__ __launch_bounds__(kScoreThreads) void scores_group_kernel(ScoreArgs a)
 {
     __shared__ Soft part[kScoreWaves];
-    __shared__ Entry lists[2][TOP ? kScoreWaves * SN_SCORES_MAX_TOP : 1];
+    __shared__ Key lists[2][TOP ? kScoreWaves * SN_SCORES_MAX_TOP : 1];
+    __shared__ Select select;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.x / a.splits;
     const int split = (int)(blockIdx.x - row * a.splits);
@@ -237,24 +396,22 @@ __global__ __launch_bounds__(kScoreThreads) void scores_group_kernel(ScoreArgs a
     Soft soft = {-INFINITY, 0.0f, 0.0f};
     TopList top;
     top.reset();
-    if (c0 < c1) scan<DT, TOP>((const char *)a.logits + row * a.stride * (DT == SN_F32 ? 4 : 2), c0, c1, wave, kScoreWaves, soft, top, a.k);
+    if (c0 < c1) scan<DT, TOP>((const char *)a.logits + row * a.stride * (DT == SN_F32 ? 4 : 2), c0, c1, wave, kScoreWaves, soft, top, a.k, lists[1] + (TOP ? wave * 64 : 0));
     soft = wave_join(soft);
     if (lane == 0) part[wave] = soft;
-    if (TOP && lane < a.k) lists[0][wave * a.k + lane] = Entry{top.v, top.i};
+    if (TOP && lane < a.k) lists[0][wave * a.k + lane] = top.key;
     __syncthreads();
     soft = join(join(part[0], part[1]), join(part[2], part[3]));
-    const Entry *best = nullptr;
-    if constexpr (TOP) best = join_lists(lists[0], lists[1], kScoreWaves, a.k);
+    Key best = kNone;
+    if constexpr (TOP) best = best_of_lists(lists[0], lists[1], kScoreWaves, a.k, select);
+    if (wave != 0) return;
     if (a.splits == 1) {
-        if (threadIdx.x == 0) write_row<DT>(a, row, soft);
-        if (TOP && (int)threadIdx.x < a.k) write_top(a, row, threadIdx.x, best[threadIdx.x].v, best[threadIdx.x].i, soft);
+        if (lane == 0) write_row<DT>(a, row, soft);
+        if constexpr (TOP) write_top<DT>(a, row, best, soft);
     } else {
-        float *dst = a.part + (row * a.splits + split) * (3 + 2 * a.k);
-        if (threadIdx.x == 0) { dst[0] = soft.m; dst[1] = soft.s; dst[2] = soft.t; }
-        if (TOP && (int)threadIdx.x < a.k) {
-            dst[3 + threadIdx.x] = best[threadIdx.x].v;
-            dst[3 + a.k + threadIdx.x] = __int_as_float(best[threadIdx.x].i);
-        }
+        float *dst = a.part + (row * a.splits + split) * (4 + 2 * a.k);
+        if (lane == 0) { dst[0] = soft.m; dst[1] = soft.s; dst[2] = soft.t; }
+        if (TOP && lane < a.k) reinterpret_cast<Key *>(dst + 4)[lane] = best;
     }
 }
 
@@ -262,28 +419,28 @@ __global__ __launch_bounds__(kScoreThreads) void scores_group_kernel(ScoreArgs a
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kScoreThreads) void scores_join_kernel(ScoreArgs a)
 {
-    extern __shared__ Entry buffers[];
-    __shared__ Soft all;
+    extern __shared__ Key buffers[];
+    __shared__ Select select;
     const int64_t row = blockIdx.x;
-    const float *src = a.part + row * a.splits * (3 + 2 * a.k);
-    if (threadIdx.x < 64) {
-        Soft s = {-INFINITY, 0.0f, 0.0f};
-        if ((int)threadIdx.x < a.splits) {
-            const float *p = src + threadIdx.x * (3 + 2 * a.k);
-            s = Soft{p[0], p[1], p[2]};
-        }
-        s = wave_join(s);
-        if (threadIdx.x == 0) { all = s; write_row<DT>(a, row, s); }
-    }
+    const int lane = threadIdx.x & 63, size = 4 + 2 * a.k;
+    const float *src = a.part + row * a.splits * size;
     if constexpr (TOP) {
         for (int e = threadIdx.x; e < a.splits * a.k; e += kScoreThreads) {
-            const int l = e / a.k, j = e - l * a.k;
-            const float *p = src + l * (3 + 2 * a.k) + 3;
-            buffers[e] = Entry{p[j], __float_as_int(p[a.k + j])};
+            const int l = e / a.k;
+            buffers[e] = reinterpret_cast<const Key *>(src + l * size + 4)[e - l * a.k];
         }
+    }
+    Soft s = {-INFINITY, 0.0f, 0.0f};
+    if (lane < a.splits) {
+        const float *p = src + lane * size;
+        s = Soft{p[0], p[1], p[2]};
+    }
+    s = wave_join(s);
+    if (threadIdx.x == 0) write_row<DT>(a, row, s);
+    if constexpr (TOP) {
         __syncthreads();
-        const Entry *best = join_lists(buffers, buffers + a.splits * a.k, a.splits, a.k);
-        if ((int)threadIdx.x < a.k) write_top(a, row, threadIdx.x, best[threadIdx.x].v, best[threadIdx.x].i, all);
+        const Key best = best_of_lists(buffers, buffers + a.splits * a.k, a.splits, a.k, select);
+        if (threadIdx.x < 64) write_top<DT>(a, row, best, s);
     }
 }
 
@@ -360,7 +517,7 @@ template <int DT, bool TOP> int launch_scores(ScoreArgs &a, hipStream_t st)
     hipLaunchKernelGGL((scores_group_kernel<DT, TOP>), dim3((unsigned)(a.rows * a.splits)), dim3(kScoreThreads), 0, st, a);
     SN_CHECK_LAUNCH("sn_label_log_probs");
     if (a.splits > 1) {
-        const size_t lds = TOP ? (size_t)2 * a.splits * a.k * sizeof(Entry) : 0;
+        const size_t lds = TOP ? (size_t)2 * a.splits * a.k * sizeof(Key) : 0;
         const int rc = sn_ensure_dynamic_lds((const void *)scores_join_kernel<DT, TOP>, lds, "sn_label_log_probs");
         if (rc != SN_OK) return rc;
         hipLaunchKernelGGL((scores_join_kernel<DT, TOP>), dim3((unsigned)a.rows), dim3(kScoreThreads), lds, st, a);
@@ -383,7 +540,7 @@ extern "C" size_t sn_label_log_probs_workspace(int64_t rows, int64_t n, int k)
 {
     if (rows < 0 || n < 1 || k < 0 || k > SN_SCORES_MAX_TOP) return 0;
     const int s = splits_for(rows, n);
-    return s > 1 ? (size_t)rows * s * (3 + 2 * k) * sizeof(float) : 16;
+    return s > 1 ? (size_t)rows * s * (4 + 2 * k) * sizeof(float) : 0;
 }
 
 extern "C" int sn_label_log_probs(const void *logits, int dtype, int64_t rows, int64_t n, int64_t row_stride, const int64_t *target, int64_t ignore_index, int k,
@@ -395,8 +552,8 @@ extern "C" int sn_label_log_probs(const void *logits, int dtype, int64_t rows, i
     SN_REQUIRE(k >= 0 && k <= SN_SCORES_MAX_TOP && k <= n, SN_ERR_BAD_ARG, "sn_label_log_probs: %d alternatives of %lld entries (at most %d)", k, (long long)n,
                SN_SCORES_MAX_TOP);
     if (rows == 0) return SN_OK;
-    SN_REQUIRE(log_probs && entropy && stats && (k == 0 || (top_log_probs && top_ids)), SN_ERR_BAD_ARG, "sn_label_log_probs: NULL pointer");
-    SN_REQUIRE(workspace && workspace_bytes >= sn_label_log_probs_workspace(rows, n, k), SN_ERR_WORKSPACE, "sn_label_log_probs: workspace of %zu bytes", workspace_bytes);
+    SN_REQUIRE(log_probs && entropy && (k == 0 || (top_log_probs && top_ids)), SN_ERR_BAD_ARG, "sn_label_log_probs: NULL pointer");
+    SN_REQUIRE(splits_for(rows, n) == 1 || (workspace && workspace_bytes >= sn_label_log_probs_workspace(rows, n, k)), SN_ERR_WORKSPACE, "sn_label_log_probs: workspace of %zu bytes", workspace_bytes);
     ScoreArgs a = {logits, rows, n, row_stride, target, ignore_index, k, splits_for(rows, n), 0, log_probs, entropy, stats, top_log_probs, top_ids, (float *)workspace};
     a.per_split = ((n + a.splits - 1) / a.splits + 7) / 8 * 8;
     const hipStream_t st = (hipStream_t)stream;

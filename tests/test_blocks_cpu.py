@@ -99,7 +99,8 @@ def test_c_entry_points_refuse(lib):
     refused(lib.sn_label_log_probs(p, 0, 1, 10, 10, p, -100, 11, p, p, p, p, p, p, 4096, None), lib, "11 alternatives")
     refused(lib.sn_label_log_probs(p, 0, 1, 100, 100, p, -100, 65, p, p, p, p, p, p, 4096, None), lib, "65 alternatives")
     refused(lib.sn_label_log_probs(p, 0, 1, 10, 10, p, -100, 2, p, p, p, None, p, p, 4096, None), lib, "NULL")
-    refused(lib.sn_label_log_probs(p, 0, 1, 10, 10, p, -100, 0, p, p, p, None, None, p, 0, None), lib, "workspace")
+    refused(lib.sn_label_log_probs(p, 0, 1, 100000, 100000, p, -100, 0, p, p, p, None, None, p, 0, None), lib, "workspace")
+    assert lib.sn_label_log_probs_workspace(1, 10, 3) == 0 and lib.sn_label_log_probs_workspace(1, 100000, 3) > 0
     refused(lib.sn_label_log_probs(p, 0, 1, 0, 10, p, -100, 0, p, p, p, None, None, p, 4096, None), lib, "n=0")
     refused(lib.sn_label_log_probs_backward(p, 0, 1, 10, 10, p, -100, p, None, None, p, None), lib, "NULL")
     assert lib.sn_label_log_probs(None, 0, 0, 10, 10, None, -100, 0, None, None, None, None, None, None, 0, None) == 0
