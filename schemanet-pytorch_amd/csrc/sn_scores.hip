@@ -149,32 +149,93 @@ struct TopList {
     }
 };
 
-// Fill an empty list from N elements a lane (x, their indexes index(u)): the k-th largest of the 64 lanes' maxima is a bound that at
-// least k elements reach; those that do are gathered and sorted.  -> false (nothing done) if more than 64 do.  room: 64 entries of
-// LDS of this wave
-template <int N, class Index> __device__ __forceinline__ bool fill_list(TopList &top, const float (&x)[N], float lane_max, Index index, int k, Key *room)
+__device__ __forceinline__ uint32_t ordered(float v)
+{
+    const uint32_t b = __float_as_uint(v);
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o ^ ((uint32_t)((int)~o >> 31) | 0x80000000u)); }
+__device__ __forceinline__ int lanes_below(uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)); }
+template <int N> __device__ __forceinline__ int count_from(const float (&x)[N], float bound)
+{
+    int count = 0;
+#pragma unroll
+    for (int u = 0; u < N; ++u) count += __popcll(__ballot(x[u] >= bound));
+    return count;
+}
+
+// The list's new state after N elements a lane (x, their indexes index(u), all behind those it has seen).  Candidates are the elements from
+// a bound on: the k-th largest of the 64 lanes' maxima for an empty list (at least k elements reach it), else what lies above the
+// list's last entry.  More than 64 of them: the bound is raised by bisection over the values' bits to the largest that k elements
+// reach; where that still leaves more than 64 - equal values - those above it and the first of the equal ones by index (EV elements of
+// a lane lie behind one another).  The candidates are gathered, sorted and merged with the list (larger of entry i and entry
+// 63 - i of the other, then the last merge of the sort).  room: 64 entries of LDS of this wave
+template <int EV, int N, class Index> __device__ __forceinline__ void absorb(TopList &top, const float (&x)[N], float lane_max, Index index, int k, Key *room)
 {
     const int lane = threadIdx.x & 63;
+    const bool empty = top.last == kNone;
     float b = lane_max;
-    wave_sort(b);
-    const float bound = fmaxf(SN_READLANE_F32(b, k - 1), kLowest);               // (never an entry at -inf)
-    int count = 0, at[N];
+    uint32_t low;
+    if (empty) {
+        wave_sort(b);
+        low = ordered(fmaxf(SN_READLANE_F32(b, k - 1), kLowest));                // (never an entry at -inf)
+    } else {
+        low = ordered(top.last_v) + 1;
+    }
+    int count = count_from(x, unordered(low));
+    if (!empty && count <= 4) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) top.offer(x[u], index(u), k);
+        return;
+    }
+    if (count > 64) {
+        uint32_t high = ordered(sn_wave_max(lane_max)) + 1;                       // under k elements reach it
+        while (high - low > 1 && count > 64) {
+            const uint32_t mid = low + (high - low) / 2;
+            const int c = count_from(x, unordered(mid));
+            if (c >= k) { low = mid; count = c; } else high = mid;
+        }
+    }
+    const float bound = unordered(low);
+    const bool equal = count > 64;                           // the bound's own value goes last
+    int at = 0;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-        const uint64_t m = __ballot(x[u] >= bound);
-        at[u] = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-        count += __popcll(m);
+        const bool in = equal ? x[u] > bound : x[u] >= bound;
+        const uint64_t m = __ballot(in);
+        if (in) room[at + lanes_below(m)] = key_of(x[u], index(u));
+        at += __popcll(m);
     }
-    if (count > 64) return false;
+    if (equal) {
 #pragma unroll
-    for (int u = 0; u < N; ++u)
-        if (x[u] >= bound) room[at[u]] = key_of(x[u], index(u));
+        for (int c = 0; c < N / EV; ++c) {
+            int before = at, all = 0;
+#pragma unroll
+            for (int e = 0; e < EV; ++e) {
+                const uint64_t m = __ballot(x[c * EV + e] == bound);
+                before += lanes_below(m);
+                all += __popcll(m);
+            }
+#pragma unroll
+            for (int e = 0; e < EV; ++e) {
+                const bool in = x[c * EV + e] == bound;
+                if (in && before < 64) room[before] = key_of(bound, index(c * EV + e));
+                before += in;
+            }
+            at += all;
+        }
+        count = 64;
+    }
     __builtin_amdgcn_wave_barrier();                         // (one wave's LDS operations stay in order)
-    top.key = lane < count ? room[lane] : kNone;
-    wave_sort(top.key);
-    if (lane >= k) top.key = kNone;
+    Key fresh = lane < count ? room[lane] : kNone;
+    wave_sort(fresh);
+    if (!empty) {
+        const Key back = ((Key)(uint32_t)__shfl((int)(fresh >> 32), 63 - lane, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)fresh, 63 - lane, 64);
+        fresh = back > top.key ? back : top.key;
+        sort_merge<64, 32>(fresh, lane);
+    }
+    top.key = lane < k ? fresh : kNone;
     top.set_last(k);
-    return true;
 }
 
 // the wave's share (segments w, w + nw, ...) of entries c0 .. c1 - 1 of a row
@@ -186,7 +247,6 @@ __device__ __forceinline__ void scan(const void *row, int64_t c0, int64_t c1, in
     const char *base = (const char *)row + c0 * (DT == SN_F32 ? 4 : 2);
     const int n = (int)(c1 - c0);
     const uint32_t fill = DT == SN_F32 ? 0xFF800000u : DT == SN_BF16 ? 0xFF80u : 0xFC00u;      // -inf
-    bool empty = true;
     for (int s0 = w * SEG; s0 < n; s0 += nw * SEG) {
         float x[16];
 #pragma unroll
@@ -217,14 +277,8 @@ __device__ __forceinline__ void scan(const void *row, int64_t c0, int64_t c1, in
         }
         if constexpr (TOP) {
             auto index = [&](int u) { return (int)c0 + s0 + ((u / EV) * 64 + lane) * EV + u % EV; };
-            if (__any(m > top.last_v)) {
-                // (m is NaN only where every element of the lane is: none of them is a candidate)
-                if (!empty || !fill_list(top, x, m == m ? m : -INFINITY, index, k, room)) {
-#pragma unroll
-                    for (int u = 0; u < 16; ++u) top.offer(x[u], index(u), k);
-                }
-                empty = false;
-            }
+            // (m is NaN only where every element of the lane is: none of them is a candidate)
+            if (__any(m > top.last_v)) absorb<EV>(top, x, m == m ? m : -INFINITY, index, k, room);
         }
     }
 }
