@@ -213,9 +213,9 @@ _BLOCK_SIGNATURES = {
     "sn_checkpoint8_weight_grad_workspace": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "sn_checkpoint8_weight_grad": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                            c_size_t, c_void_p]),
-    "sn_block_norms_forward": (c_int, [POINTER(BlockNormsArgs), c_void_p]),
+    "sn_block_norms_forward": (c_int, [c_void_p, c_void_p]),          # (a BlockNormsArgs by reference, or its bytes)
     "sn_block_norms_workspace": (c_size_t, [c_int64, c_int]),
-    "sn_block_norms_backward": (c_int, [POINTER(BlockNormsArgs), c_void_p]),
+    "sn_block_norms_backward": (c_int, [c_void_p, c_void_p]),
     "sn_label_log_probs_workspace": (c_size_t, [c_int64, c_int64, c_int]),
     "sn_label_log_probs": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_size_t, c_void_p]),

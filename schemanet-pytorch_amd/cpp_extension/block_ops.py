@@ -6,8 +6,8 @@ They take CUDA tensors in float32, bfloat16 or float16 with rows of any stride, 
 once; outputs are new contiguous tensors; nothing synchronises, all of them can be captured into a graph.  Under `torch.autocast`
 their floating-point inputs are cast to float32, like those of the other HIP-backed ops of this package.  Arguments that do not
 fit raise RuntimeError before anything is launched."""
+import struct
 from collections import namedtuple
-from ctypes import byref
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -36,7 +36,7 @@ def _one_device(*ts):
 
 
 def _p(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -70,6 +70,8 @@ def _once(backward):
 
 def _rows(t, width):
     """[..., width] as (tensor that holds the rows, stride of a row): a view where the rows lie evenly apart, a copy otherwise"""
+    if t.is_contiguous():
+        return t, width
     if t.stride(-1) != 1 and width > 1:
         t = t.contiguous()
     if t.dim() == 2:
@@ -226,112 +228,102 @@ def linear_checkpoint8(x, weight, bias=None):
 
 
 # ------------------------------------------------------------- the end of a residual block and the norm before the next one
-def _norm_args(x, branch, gate, scale, post, pre, rms, eps, n_valid):
-    width = x.shape[-1]
-    a = N.BlockNormsArgs()
-    a.dtype, a.rms, a.width, a.eps = _TYPES[x.dtype], int(rms), width, eps
-    a.rows = x.numel() // width
-    a.rows_per_graph = x.shape[1] if n_valid is not None else 0
-    a.n_valid = _p(n_valid)
-    params = [t for t in (scale, *post, *pre) if t is not None]
-    a.param_dtype = _TYPES[params[0].dtype] if params else 0
-    a.has_post, a.has_pre = int(post[0] is not None), int(pre[0] is not None)
-    a.scale, a.post_weight, a.post_bias, a.pre_weight, a.pre_bias = _p(scale), _p(post[0]), _p(post[1]), _p(pre[0]), _p(pre[1])
-    return a
+# sn_block_norms_args as one packed value (N.BlockNormsArgs names its members): setting 45 members one by one is a sixth of a small call
+_NORM_ARGS = struct.Struct("@IiiiqiiPfiiPPPqqqPPPPPPPPPPPPPPPPqqPPPPPPPPPN")
 
 
-def _norms_forward(x, branch, gate, scale, post, pre, rms, eps, n_valid, train, keep8):
-    lib = _library()
+def _norms_forward(x, branch, gate, params, rms, eps, n_valid, train, keep8):
+    """-> y, h, row statistics (train), checkpoints of x, branch and gate (train and keep8)"""
+    scale, post_w, post_b, pre_w, pre_b = params
     dev, width = x.device, x.shape[-1]
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if pre[0] is not None else None
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if pre_w is not None else None
     stats, kept = None, ()
-    if x.numel() == 0:
+    rows = x.numel() // width
+    if rows == 0:
         return y, h, stats, kept
-    a = _norm_args(x, branch, gate, scale, post, pre, rms, eps, n_valid)
-    vx, a.x_stride = _rows(x, width)
-    vb, a.branch_stride = _rows(branch, width)
-    a.x, a.branch = _p(vx), _p(vb)
-    if gate is not None:
-        vg, a.gate_stride = _rows(gate, width)
-        a.gate = _p(vg)
-    a.y, a.h = _p(y), _p(h)
+    vx, sx = _rows(x, width)
+    vb, sb = _rows(branch, width)
+    vg, sg = _rows(gate, width) if gate is not None else (None, 0)
+    codes = (0,) * 6
     if train:
-        stats = torch.empty((a.rows, 4), dtype=torch.float32, device=dev)
-        a.stats = _p(stats)
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
         if keep8:
-            kept = tuple(None if t is None else _empty_checkpoint((a.rows, width), x.dtype, dev) for t in (x, branch, gate))
-            a.x_codes, a.x_exps = _p(kept[0].codes), _p(kept[0].exps)
-            a.branch_codes, a.branch_exps = _p(kept[1].codes), _p(kept[1].exps)
-            if gate is not None:
-                a.gate_codes, a.gate_exps = _p(kept[2].codes), _p(kept[2].exps)
-    _launch(lib.sn_block_norms_forward, "sn_block_norms_forward", dev, byref(a))
+            kept = tuple(None if t is None else _empty_checkpoint((rows, width), x.dtype, dev) for t in (x, branch, gate))
+            codes = [0 if k is None else t.data_ptr() for k in kept for t in ((k.codes, k.exps) if k is not None else (None, None))]
+    args = _NORM_ARGS.pack(_NORM_ARGS.size, _TYPES[x.dtype], _param_type(params), rms, rows, width, 0 if n_valid is None else x.shape[1], _p(n_valid), eps,
+                           post_w is not None, pre_w is not None, _p(vx), _p(vb), _p(vg), sx, sb, sg, _p(scale), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b),
+                           _p(y), _p(h), _p(stats), *codes, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _launch(_library().sn_block_norms_forward, "sn_block_norms_forward", dev, args)
     return y, h, stats, kept
+
+
+def _param_type(params):
+    for t in params:
+        if t is not None:
+            return _TYPES[t.dtype]
+    return 0
 
 
 class _GatedResidualNorms(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, gate, scale, post_w, post_b, pre_w, pre_b, rms, eps, n_valid, keep8):
-        x, branch = x.detach(), branch.detach()
-        y, h, stats, kept = _norms_forward(x, branch, gate, scale, (post_w, post_b), (pre_w, pre_b), rms, eps, n_valid, True, keep8)
+        params = (scale, post_w, post_b, pre_w, pre_b)
+        y, h, stats, kept = _norms_forward(x, branch, gate, params, rms, eps, n_valid, True, keep8)
         if kept:
             held = [t for k in kept for t in ((k.codes, k.exps) if k is not None else (None, None))]
         else:
             held = [x, branch, gate]
-        ctx.save_for_backward(scale, post_w, post_b, pre_w, pre_b, n_valid, stats, *held)
-        ctx.opts, ctx.kept = (tuple(x.shape), x.dtype, rms, eps), bool(kept)
+        ctx.save_for_backward(*params, n_valid, stats, *held)
+        ctx.opts = (x.shape, x.dtype, rms, eps, bool(kept))
         ctx.set_materialize_grads(False)
         return y if h is None else (y, h)
 
     @_once
     def backward(ctx, dy, dh=None):
         scale, post_w, post_b, pre_w, pre_b, n_valid, stats, *held = ctx.saved_tensors
-        shape, dtype, rms, eps = ctx.opts
+        shape, dtype, rms, eps, kept = ctx.opts
         width, dev = shape[-1], (dy if dy is not None else dh).device
         want = ctx.needs_input_grad
         params = (scale, post_w, post_b, pre_w, pre_b)
         if stats is None:                                                   # no rows
             whole = [torch.zeros(shape, dtype=dtype, device=dev) if want[i] else None for i in range(3)]
             return (*whole, *(torch.zeros_like(p) if p is not None and want[3 + i] else None for i, p in enumerate(params)), None, None, None, None)
-        lib = _library()
-        x_like = torch.empty(shape, dtype=dtype, device=dev)                # dx, or only the sizes
-        a = _norm_args(x_like, None, None, scale, (post_w, post_b), (pre_w, pre_b), rms, eps, n_valid)
-        a.stats = _p(stats)
-        if ctx.kept:
-            a.x_codes, a.x_exps, a.branch_codes, a.branch_exps, a.gate_codes, a.gate_exps = (_p(t) for t in held)
+        rows = stats.shape[0]
+        codes = vx = vb = vg = None
+        sx = sb = sg = 0
+        if kept:
+            codes = [_p(t) for t in held]
             gated = held[4] is not None
         else:
-            x, branch, gate = held
-            vx, a.x_stride = _rows(x, width)
-            vb, a.branch_stride = _rows(branch, width)
-            a.x, a.branch = _p(vx), _p(vb)
-            gated = gate is not None
+            vx, sx = _rows(held[0], width)
+            vb, sb = _rows(held[1], width)
+            gated = held[2] is not None
             if gated:
-                vg, a.gate_stride = _rows(gate, width)
-                a.gate = _p(vg)
-        if dy is not None:
-            vy, a.dy_stride = _rows(dy, width)
-            a.dy = _p(vy)
-        if dh is not None:
-            vh, a.dh_stride = _rows(dh, width)
-            a.dh = _p(vh)
-        dx = x_like if want[0] else None
-        dbranch = torch.empty_like(x_like) if want[1] else None
-        dgate = torch.empty_like(x_like) if gated and want[2] else None
-        a.dx, a.dbranch, a.dgate = _p(dx), _p(dbranch), _p(dgate)
-        grads = [torch.empty_like(p) if p is not None and want[3 + i] else None for i, p in enumerate(params)]
+                vg, sg = _rows(held[2], width)
+        vy, sy = _rows(dy, width) if dy is not None else (None, 0)
+        vh, sh = _rows(dh, width) if dh is not None else (None, 0)
+        dx = torch.empty(shape, dtype=dtype, device=dev) if want[0] else None
+        dbranch = torch.empty(shape, dtype=dtype, device=dev) if want[1] else None
+        dgate = torch.empty(shape, dtype=dtype, device=dev) if gated and want[2] else None
+        columns = [p is not None and want[3 + i] for i, p in enumerate(params)]
+        grads = [None] * 5
+        if any(columns):
+            lines = torch.empty((5, width), dtype=next(p.dtype for p in params if p is not None), device=dev).unbind(0)
+            grads = [lines[i] if c else None for i, c in enumerate(columns)]
+        into = [_p(g) for g in grads]
         if dh is None:                                                      # the norm before the next block took no part
             for i in (3, 4):
+                into[i] = 0
                 if grads[i] is not None:
                     grads[i].zero_()
-            a.dpre_weight = a.dpre_bias = None
-        else:
-            a.dpre_weight, a.dpre_bias = _p(grads[3]), _p(grads[4])
-        a.dscale, a.dpost_weight, a.dpost_bias = _p(grads[0]), _p(grads[1]), _p(grads[2])
-        size = lib.sn_block_norms_workspace(a.rows, width)
+        lib = _library()
+        size = lib.sn_block_norms_workspace(rows, width)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = _p(ws), size
-        _launch(lib.sn_block_norms_backward, "sn_block_norms_backward", dev, byref(a))
+        args = _NORM_ARGS.pack(_NORM_ARGS.size, _TYPES[dtype], _param_type(params), rms, rows, width, 0 if n_valid is None else shape[1], _p(n_valid), eps,
+                               post_w is not None, pre_w is not None, _p(vx), _p(vb), _p(vg), sx, sb, sg, _p(scale), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b),
+                               0, 0, _p(stats), *(codes or (0,) * 6), _p(vy), _p(vh), sy, sh, _p(dx), _p(dbranch), _p(dgate), *into, _p(ws), size)
+        _launch(lib.sn_block_norms_backward, "sn_block_norms_backward", dev, args)
         return (dx, dbranch, dgate, *grads, None, None, None, None)
 
 
@@ -380,7 +372,7 @@ def gated_residual_norms(x, branch, gate=None, scale=None, post=None, pre=None, 
     if _wants_grad(x, branch, gate, *params):
         out = _GatedResidualNorms.apply(x, branch, gate, *params, norm == "rms", float(eps), n_valid, bool(checkpoint8))
         return out if norms[2] is not None else (out, None)
-    return _norms_forward(x, branch, gate, params[0], params[1:3], params[3:5], norm == "rms", float(eps), n_valid, False, False)[:2]
+    return _norms_forward(x, branch, gate, params, norm == "rms", float(eps), n_valid, False, False)[:2]
 
 
 # -------------------------------------------------------------------------------- log probabilities of given tokens
