@@ -27,11 +27,14 @@ def _need(ok, message, *args):
 def _one_device(*ts):
     dev = None
     for t in ts:
-        if t is None:
-            continue
-        _need(t.is_cuda, "expected CUDA tensors (the HIP path has no CPU fallback)")
-        dev = dev or t.device
-        _need(t.device == dev, "tensors on different devices: {} vs {}", t.device, dev)
+        if t is not None:
+            d = t.device
+            if dev is None:
+                dev = d
+                _need(d.type == "cuda", "expected CUDA tensors (the HIP path has no CPU fallback)")
+            elif d != dev:
+                _need(d.type == "cuda", "expected CUDA tensors (the HIP path has no CPU fallback)")
+                _need(False, "tensors on different devices: {} vs {}", d, dev)
     return dev
 
 
@@ -94,7 +97,11 @@ def _autocast(*ts):
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ------------------------------------------------------------------------------------------- activations kept in 8 bits
@@ -342,36 +349,46 @@ def gated_residual_norms(x, branch, gate=None, scale=None, post=None, pre=None, 
     gradient's formulas at the kept values, with the row statistics of the forward pass.
 
     Differentiable in x, branch, gate and all parameters."""
-    _need(norm in ("layer", "rms"), "gated_residual_norms: norm must be 'layer' or 'rms', got {!r}", norm)
-    _need(torch.is_tensor(x) and x.dtype in _TYPES and x.dim() >= 1, "gated_residual_norms: expected a float32, bfloat16 or float16 tensor")
-    x, branch, gate, scale = _autocast(x, branch, gate, scale)
-    width = x.shape[-1]
-    _need(1 <= width <= MAX_NORM_WIDTH, "gated_residual_norms: width {} outside 1 .. {}", width, MAX_NORM_WIDTH)
-    for t, name in ((branch, "branch"), (gate, "gate")):
-        _need(t is None and name == "gate" or torch.is_tensor(t) and t.dtype == x.dtype and t.shape == x.shape,
-              "gated_residual_norms: {} must have x's shape {} and type", name, tuple(x.shape))
-    norms = []
-    for pair, name in ((post, "post"), (pre, "pre")):
-        if pair is None:
-            norms += [None, None]
-            continue
-        _need(len(pair) == 2 and torch.is_tensor(pair[0]), "gated_residual_norms: {} must be (weight, bias or None)", name)
-        norms += list(_autocast(*pair))
-    params = [scale] + norms
-    for t in params:
-        _need(t is None or torch.is_tensor(t) and t.dtype in _TYPES and tuple(t.shape) == (width,), "gated_residual_norms: parameters must be [{}]", width)
-    _need(eps >= 0, "gated_residual_norms: eps {}", eps)
-    if n_valid is not None:
-        _need(x.dim() == 3 and n_valid.dtype == torch.int32 and tuple(n_valid.shape) == (x.shape[0],) and n_valid.is_contiguous(),
-              "gated_residual_norms: n_valid must be int32 [G] with x [G, n, width]")
+    # (plain tests: a message is only put together where one fails)
+    if norm != "layer" and norm != "rms":
+        _need(False, "gated_residual_norms: norm must be 'layer' or 'rms', got {!r}", norm)
+    if not torch.is_tensor(x) or x.dtype not in _TYPES or x.dim() < 1:
+        _need(False, "gated_residual_norms: expected a float32, bfloat16 or float16 tensor")
+    autocast = torch.is_autocast_enabled("cuda")
+    if autocast:
+        x, branch, gate, scale = _autocast(x, branch, gate, scale)
+    dtype, shape = x.dtype, x.shape
+    width = shape[-1]
+    if not 1 <= width <= MAX_NORM_WIDTH:
+        _need(False, "gated_residual_norms: width {} outside 1 .. {}", width, MAX_NORM_WIDTH)
+    if not torch.is_tensor(branch) or branch.dtype != dtype or branch.shape != shape:
+        _need(False, "gated_residual_norms: branch must have x's shape {} and type", tuple(shape))
+    if gate is not None and (not torch.is_tensor(gate) or gate.dtype != dtype or gate.shape != shape):
+        _need(False, "gated_residual_norms: gate must have x's shape {} and type", tuple(shape))
+    params = [scale, None, None, None, None]
+    for at, pair in ((1, post), (3, pre)):
+        if pair is not None:
+            if len(pair) != 2 or not torch.is_tensor(pair[0]):
+                _need(False, "gated_residual_norms: {} must be (weight, bias or None)", "post" if at == 1 else "pre")
+            params[at], params[at + 1] = _autocast(*pair) if autocast else pair
+    types = None
+    for i, t in enumerate(params):
+        if t is not None:
+            if not torch.is_tensor(t) or t.dtype not in _TYPES or t.dim() != 1 or t.shape[0] != width:
+                _need(False, "gated_residual_norms: parameters must be [{}]", width)
+            types = t.dtype if types is None or types == t.dtype else torch.float64       # (float64: mixed)
+            if not t.is_contiguous():
+                params[i] = t.contiguous()
+    if eps < 0:
+        _need(False, "gated_residual_norms: eps {}", eps)
+    if n_valid is not None and not (x.dim() == 3 and n_valid.dtype == torch.int32 and n_valid.shape == shape[:1] and n_valid.is_contiguous()):
+        _need(False, "gated_residual_norms: n_valid must be int32 [G] with x [G, n, width]")
     _one_device(x, branch, gate, n_valid, *params)
-    types = {t.dtype for t in params if t is not None}
-    if len(types) > 1:
+    if types == torch.float64:
         params = [None if t is None else t.float() for t in params]
-    params = [t if t is None or t.is_contiguous() else t.contiguous() for t in params]
     if _wants_grad(x, branch, gate, *params):
         out = _GatedResidualNorms.apply(x, branch, gate, *params, norm == "rms", float(eps), n_valid, bool(checkpoint8))
-        return out if norms[2] is not None else (out, None)
+        return out if pre is not None else (out, None)
     return _norms_forward(x, branch, gate, params, norm == "rms", float(eps), n_valid, False, False)[:2]
 
 
@@ -437,12 +454,15 @@ def label_log_probs(logits, target, topk=0, ignore_index=-100):
         top_log_probs, top_ids [..., topk]: the topk largest, the lowest index first among equals (None for topk = 0; at most 64)
     log_probs and entropy are differentiable in the logits, the alternatives are not.  A row of -inf only has no distribution: log_probs
     and top_log_probs -inf, entropy 0, no gradient.  A NaN or +inf logit makes its row's results NaN."""
-    _need(torch.is_tensor(logits) and logits.dtype in _TYPES and logits.dim() >= 1, "label_log_probs: expected float32, bfloat16 or float16 logits")
-    _need(torch.is_tensor(target) and target.dtype == torch.int64 and target.shape == logits.shape[:-1],
-          "label_log_probs: expected an int64 target of shape {}", tuple(logits.shape[:-1]))
+    if not torch.is_tensor(logits) or logits.dtype not in _TYPES or logits.dim() < 1:
+        _need(False, "label_log_probs: expected float32, bfloat16 or float16 logits")
+    if not torch.is_tensor(target) or target.dtype != torch.int64 or target.shape != logits.shape[:-1]:
+        _need(False, "label_log_probs: expected an int64 target of shape {}", tuple(logits.shape[:-1]))
     n, topk = logits.shape[-1], int(topk)
-    _need(1 <= n < 1 << 30 and target.numel() < 1 << 24, "label_log_probs: {} rows of {} entries", target.numel(), n)
-    _need(0 <= topk <= min(n, MAX_ALTERNATIVES), "label_log_probs: {} alternatives of {} entries (at most {})", topk, n, MAX_ALTERNATIVES)
+    if not (1 <= n < 1 << 30 and target.numel() < 1 << 24):
+        _need(False, "label_log_probs: {} rows of {} entries", target.numel(), n)
+    if not 0 <= topk <= min(n, MAX_ALTERNATIVES):
+        _need(False, "label_log_probs: {} alternatives of {} entries (at most {})", topk, n, MAX_ALTERNATIVES)
     _one_device(logits, target)
     logits, = _autocast(logits)
     target = target.contiguous()
