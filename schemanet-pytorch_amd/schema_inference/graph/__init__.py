@@ -364,6 +364,16 @@ class SchemaNetPredictor(nn.Module):
         while in_flight:
             yield hand_over(in_flight.popleft())
 
+    def answers(self, x: torch.Tensor, topk: int = 5, label: torch.Tensor = None):
+        """`forward(x)` as answers: the `topk` most likely classes of every image with their log probabilities and the entropy of its
+        distribution over the classes; with `label` [bs] also the log probability of the given classes (otherwise None).
+        -> ops.LabelLogProbs(log_probs, entropy, top_log_probs, top_ids)"""
+        from cpp_extension import ops
+        pred = self.forward(x)["pred"]
+        given = torch.full(pred.shape[:1], -100, dtype=torch.int64, device=pred.device) if label is None else label
+        out = ops.label_log_probs(pred, given, topk=min(int(topk), pred.shape[-1]))
+        return out if label is not None else out._replace(log_probs=None)
+
     def forward(self, x: torch.Tensor, requires_graph: bool = False) -> Dict[str, torch.Tensor]:
         wrapper = self.ingredient_wrapper
         if (self.graph_replay and not self.training and not requires_graph and not torch.is_grad_enabled()

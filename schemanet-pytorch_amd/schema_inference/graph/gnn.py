@@ -145,15 +145,41 @@ class Layer(nn.Module):
         return self.activation(self.norm(feat))
 
 
-class GNN(nn.Module):
-    def __init__(self, num_codes: int, embed_dim: int, num_layers: int, identity_proj: bool = False,
-                 activation: str = "relu"):
+class ResidualLayer(nn.Module):
+    """One block of a deep residual GNN: h -> convolution -> activation is the branch, which comes back to the stream through its own
+    norm, a gate computed from h and a learned scale for each feature:
+        x <- x + scale * sigmoid(gate(h)) * post(act(g_conv(h))),    h <- norm of the next block (x)
+    `norm` is the norm before this block."""
+
+    def __init__(self, emb_dim: int, activation: str, identity_proj: bool = False, scale_init: float = 0.1):
         super().__init__()
+        self.norm = nn.LayerNorm(emb_dim)
+        self.g_conv = GraphConv(emb_dim, emb_dim, identity_proj)
+        self.activation = get_activation_fn(activation)
+        self.gate = nn.Linear(emb_dim, emb_dim)
+        self.post = nn.LayerNorm(emb_dim)
+        self.scale = nn.Parameter(torch.full((emb_dim,), float(scale_init)))
+
+
+class GNN(nn.Module):
+    """residual=True (no reference counterpart; the default is the reference's GNN, parameter for parameter): the layers are
+    `ResidualLayer`s, for depths at which plain ones stop training.  The end of a block and the norm before the next one are one pass
+    (`ops.gated_residual_norms`).  checkpoint8=True: what the backward pass keeps of a block - the input of both Linears, stream,
+    branch and gate - is kept in 8 bits (`ops.checkpoint8`), 1.03 bytes an element instead of 4."""
+
+    def __init__(self, num_codes: int, embed_dim: int, num_layers: int, identity_proj: bool = False,
+                 activation: str = "relu", residual: bool = False, checkpoint8: bool = False):
+        super().__init__()
+        if checkpoint8 and not residual:
+            raise ValueError("GNN: checkpoint8 needs residual=True")
+        self.residual, self.checkpoint8 = bool(residual), bool(checkpoint8)
         self.num_codes = num_codes
         self.embed_dim = embed_dim
         self.num_layers = num_layers
         self.embedding = nn.Embedding(num_codes + 1, embed_dim, padding_idx=num_codes)
-        self.layers = nn.ModuleList([Layer(embed_dim, activation, identity_proj) for _ in range(num_layers)])
+        self.layers = nn.ModuleList([(ResidualLayer if residual else Layer)(embed_dim, activation, identity_proj) for _ in range(num_layers)])
+        if residual:
+            self.out_norm = nn.LayerNorm(embed_dim)
         self._prepared = None
         self.fc = nn.Linear(embed_dim, embed_dim)
         nn.init.normal_(self.fc.weight)
@@ -196,7 +222,7 @@ class GNN(nn.Module):
         activation: embed_dim 256 (the shipped CIFAR / Caltech configurations) with every elementwise step fused into
         the GEMM epilogues, other widths that are a multiple of 16 (1024 in the ImageNet yaml) with the same GEMMs and
         the LayerNorm / pooling kernels of the library route in between."""
-        if os.environ.get("SN_GCN_MFMA", "1") == "0" or self.embed_dim % 16 != 0 or len(self.layers) != 2:
+        if self.residual or os.environ.get("SN_GCN_MFMA", "1") == "0" or self.embed_dim % 16 != 0 or len(self.layers) != 2:
             return False
         return all(isinstance(l.g_conv.linear, nn.Linear) and (l._is_relu or l._is_none) for l in self.layers)
 
@@ -265,7 +291,7 @@ class GNN(nn.Module):
     def train_folds(self, device_is_cuda: bool = True) -> bool:
         """True when `forward` under autograd takes the route with layer 1's Linear folded into the embedding table"""
         first = self.layers[0] if len(self.layers) else None
-        return bool(device_is_cuda and first is not None and isinstance(first.g_conv.linear, nn.Linear) and self.embed_dim % 16 == 0
+        return bool(not self.residual and device_is_cuda and first is not None and isinstance(first.g_conv.linear, nn.Linear) and self.embed_dim % 16 == 0
                     and self.embedding.weight.is_cuda and self.embedding.weight.dtype == torch.float32
                     and os.environ.get("SN_GCN_MFMA", "1") != "0" and os.environ.get("SN_TRAIN_FOLD", "1") != "0")
 
@@ -374,6 +400,44 @@ class GNN(nn.Module):
                                              divisor_dev=divisor)                                    # (nor H2)
         return ops.pool_fc(pooled, 1.0, self.fc.weight, self.fc.bias, weight_t=prepared.get("fc_t"))    # (the final Linear without a library GEMM)
 
+    def _residual_linear(self, lin, x):
+        if not isinstance(lin, nn.Linear):
+            return lin(x)
+        if x.is_cuda and x.dtype == torch.float32 and lin.in_features % 16 == 0 and lin.out_features % 16 == 0 and x.numel() > 0:
+            if self.checkpoint8 and torch.is_grad_enabled() and (x.requires_grad or lin.weight.requires_grad):
+                return ops.linear_checkpoint8(x, lin.weight, lin.bias)
+            return ops.linear_mfma(x, lin.weight, lin.bias)
+        return lin(x)
+
+    def _forward_residual(self, nodes, edges, ingredients, n_valid, divisor):
+        """The residual form of `forward` (inference and training alike): the stream x and its normed form h go from block to block"""
+        x = self._embed(ingredients)
+        G, n, E = x.shape
+        # one adjacency operand for all blocks (and for their backward passes); the products' edge gradients are summed, as in the
+        # plain layers
+        planes = ops.gcn_adjacency_planes(_contig(edges.detach())) if edges.is_cuda and E % 16 == 0 and os.environ.get("SN_GCN_MFMA", "1") != "0" else None
+        adj = None if planes is not None else GraphConv.adjacency(edges)
+        first = self.layers[0].norm if len(self.layers) else self.out_norm
+        if E <= 1024 and x.is_cuda:
+            h = ops.mask_layernorm_act(x, first.weight, first.bias, first.eps, n_valid=n_valid, relu=False)
+            if n_valid is not None:
+                # (that op norms a padding row as a row of zeros: its bias; here padding is zero throughout)
+                h = h.masked_fill((torch.arange(n, device=h.device)[None, :] >= n_valid[:, None])[..., None], 0.0)
+        else:
+            h = first(x)
+        for i, layer in enumerate(self.layers):
+            summed = ops.edges_adj_matmul(edges, h, planes, True) if planes is not None else torch.bmm(adj, h)
+            branch = layer.activation(self._residual_linear(layer.g_conv.linear, summed))
+            gate = self._residual_linear(layer.gate, h)
+            after = self.layers[i + 1].norm if i + 1 < len(self.layers) else self.out_norm
+            x, h = ops.gated_residual_norms(x, branch, gate=gate, scale=layer.scale, post=(layer.post.weight, layer.post.bias),
+                                            pre=(after.weight, after.bias), norm="layer", eps=after.eps, n_valid=n_valid, checkpoint8=self.checkpoint8)
+        if self._differentiable(nodes, edges):
+            pooled = ops.weighted_pool_autograd(h, nodes, divisor) if E % 4 == 0 else (h * nodes[..., None]).sum(dim=1) / (n if divisor is None else divisor)
+        else:
+            pooled = ops.weighted_pool(h, nodes, divisor)
+        return self._residual_linear(self.fc, pooled)
+
     def forward(self, nodes: torch.Tensor, edges: torch.Tensor, ingredients: torch.LongTensor,
                 feat_mask: torch.BoolTensor = None, n_valid: torch.Tensor = None,
                 divisor: Optional[torch.Tensor] = None, adjacency=None, prepared=None, compact=None) -> torch.Tensor:
@@ -392,6 +456,8 @@ class GNN(nn.Module):
         fused = nodes.is_cuda and not self._differentiable(nodes, edges)
         if n_valid is None and feat_mask is not None:
             n_valid = (~feat_mask).sum(dim=1).to(torch.int32)   # masks are suffix masks (match.py:48-51)
+        if self.residual:
+            return self._forward_residual(nodes, edges, ingredients, n_valid, divisor)
         if fused and self._mfma_ok():
             run = self._forward_mfma if self.embed_dim == 256 else self._forward_mfma_wide
             return run(nodes, edges, ingredients, n_valid, divisor, prepared=prepared)

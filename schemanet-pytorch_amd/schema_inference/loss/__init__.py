@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-__all__ = ["Loss", "CELoss", "SchemaInferenceLoss", "get_loss_fn", "entropy", "rectify_linear"]
+__all__ = ["Loss", "CELoss", "CEEntropyLoss", "SchemaInferenceLoss", "get_loss_fn", "entropy", "rectify_linear"]
 __path__ = extend_path(__path__, __name__)      # `schema_inference.loss.<submodule>` of a reference checkout behind us still resolves
 
 
@@ -67,6 +67,31 @@ class CELoss(Loss):
         return OrderedDict([(name, self.loss_fn(_logits_of(output), target["label"]))])
 
 
+class CEEntropyLoss(Loss):
+    """Cross entropy and the mean entropy of the answers, for loss weights on both (a negative weight on "entropy" keeps a classifier from
+    growing too sure of itself):  cls = -mean over the labelled rows of log p[label],  entropy = mean over those rows of -sum p log p.
+    On the GPU both and their gradient are one pass over the scores each way (`cpp_extension.ops.label_log_probs`)."""
+
+    def __init__(self, ignore_index: int = -100, **kwargs):
+        super().__init__()
+        self.ignore_index = ignore_index
+
+    def forward(self, output, target):
+        scores, label = _logits_of(output), target["label"]
+        used = label != self.ignore_index
+        if scores.is_cuda:
+            from cpp_extension import ops
+            got = ops.label_log_probs(scores, label, ignore_index=self.ignore_index)
+            log_probs, ent = got.log_probs, got.entropy
+        else:
+            lp = torch.log_softmax(scores.float(), dim=-1)
+            log_probs = lp.gather(-1, label.masked_fill(~used, 0).unsqueeze(-1)).squeeze(-1) * used
+            p = lp.exp()
+            ent = -(p * lp.masked_fill(p == 0, 0.0)).sum(-1)
+        count = used.sum()
+        return OrderedDict([("cls", -log_probs.sum() / count), ("entropy", (ent * used).sum() / count)])
+
+
 class SchemaInferenceLoss(Loss):
     def __init__(self, re_a_vertex: float = 3, re_a_edge: float = 3, **kwargs):
         super().__init__()
@@ -85,7 +110,7 @@ class SchemaInferenceLoss(Loss):
         return ret
 
 
-_REGISTRY = {"ce_loss": CELoss, "schema_inference_loss": SchemaInferenceLoss}
+_REGISTRY = {"ce_loss": CELoss, "ce_entropy_loss": CEEntropyLoss, "schema_inference_loss": SchemaInferenceLoss}
 
 
 def get_loss_fn(loss_cfg: Dict[str, Any], **kwargs) -> Loss:

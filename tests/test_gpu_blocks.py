@@ -558,7 +558,7 @@ def test_a_training_step_of_all_of_them(ops):
     ent = -(lp.exp() * lp).sum(-1) * used
     loss = -(picked.sum() + 0.1 * ent.sum()) / used.sum() + 1e-3 * y.square().mean()
     want = torch.autograd.grad(loss, [ref[k] for k in ("x", "w", "b", "gate", "scale", "pw", "pb", "qw", "qb", "head")])
-    assert abs(float(got[0]) - float(loss)) <= 1e-5 * abs(float(loss))
+    assert abs(float(got[0].detach()) - float(loss.detach())) <= 1e-5 * abs(float(loss.detach()))
     for a, b in zip(got[1:], want):
         assert float((a.double() - b).norm() / b.norm()) < 0.05
 
