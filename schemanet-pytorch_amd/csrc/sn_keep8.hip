@@ -41,39 +41,43 @@ __global__ __launch_bounds__(kPackThreads) void checkpoint8_kernel(const void *x
 template <int DT>
 __global__ __launch_bounds__(kPackThreads) void restore8_kernel(const uint8_t *codes, const uint8_t *exps, int64_t rows, int n, void *out)
 {
-    const int npad = (n + 31) & ~31, groups = (n + 7) / 8;
+    constexpr int EV = DT == SN_F32 ? 4 : 8;                 // 16 bytes of the result a lane
+    const int npad = (n + 31) & ~31, groups = (n + EV - 1) / EV;
     const int64_t total = rows * groups, turn = (int64_t)gridDim.x * kPackThreads;
     for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < total; i += turn) {
         const int64_t r = total <= 0xFFFFFFFFll ? (int64_t)((uint32_t)i / (uint32_t)groups) : i / groups;
-        const int j = (int)(i - r * groups) * 8;
-        const uint2 c = *reinterpret_cast<const uint2 *>(codes + r * npad + j);
-        const uint32_t q[2] = {c.x, c.y};
-        float v[8];
-        decode<8>(v, q, exps[r * (npad / 32) + j / 32]);
-        store_row<DT, 8>((char *)out + r * n * (DT == SN_F32 ? 4 : 2), j, n, v);
+        const int j = (int)(i - r * groups) * EV;
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(codes + r * npad + j);
+        uint32_t q[EV / 4];
+#pragma unroll
+        for (int k = 0; k < EV / 4; ++k) q[k] = src[k];
+        float v[EV];
+        decode<EV>(v, q, exps[r * (npad / 32) + j / 32]);
+        store_row<DT, EV>((char *)out + r * n * (DT == SN_F32 ? 4 : 2), j, n, v);
     }
 }
 
 // ------------------------------------------------------------------------------------------
 // dW: a workgroup owns TILE x TILE outputs of one split of the summed rows, BK rows a step, MFMA 32x32x16 on wave tiles of
-// 128 x 64 (TILE 256, eight waves) or 64 x 64 (TILE 128, four).  Both operands lie with the summed index outermost, so a
+// 128 x 64 (TILE 256) or 64 x 32 (TILE 128) of eight waves.  Both operands lie with the summed index outermost, so a
 // staging thread takes 8 rows of UC columns, turns them in registers (the bf16 conversion pairs two ROWS into a word) and
 // writes 8 consecutive rows of one column to LDS, as the matrix instruction wants them.  Half of the waves stage dY, the other
 // half the kept codes; two LDS buffers, one barrier a step; the dY waves stage before their products and the code waves after
 // them, so that on every SIMD the vector work of one wave runs under the matrix instructions of the other.
 typedef uint32_t u32;
 
+template <int V> struct Type { static constexpr int value = V; };
 template <int DT> constexpr int pieces() { return DT == SN_F32 ? 3 : DT == SN_F16 ? 2 : 1; }
 
 template <int DT, int TILE> struct Grad {
     static constexpr int P = pieces<DT>();
-    static constexpr int BK = P == 1 ? 64 : 32;              // rows of a step: two buffers of P + 1 pieces in 128 KiB
-    static constexpr int UC = P == 1 ? 8 : 4;                // columns of a staging thread
-    static constexpr int kWaves = TILE == 256 ? 8 : 4, kThreads = kWaves * 64;
+    static constexpr int BK = TILE == 128 || P == 1 ? 64 : 32;       // rows of a step: two buffers of P + 1 pieces in 128 KiB
+    static constexpr int UC = TILE == 256 && P == 1 ? 8 : 4; // columns of a staging thread
+    static constexpr int kWaves = 8, kThreads = kWaves * 64;
     static constexpr int kPlane = TILE * BK;                 // bf16 elements of one piece
     static constexpr int kBuffer = (P + 1) * kPlane;
     static constexpr int kGroups = TILE / UC;                // column groups
-    static constexpr int MT = TILE == 256 ? 4 : 2, NT = 2;   // 32 x 32 products of a wave
+    static constexpr int MT = TILE == 256 ? 4 : 2, NT = TILE == 256 ? 2 : 1;     // 32 x 32 products of a wave
     static constexpr int kBlocks = TILE / 32;                // checkpoint blocks of a row of the tile
     static constexpr int kKg = 64 / kGroups > 0 ? 64 / kGroups : 1;      // row groups of a staging wave
     static constexpr int JR = 64 / (kKg * kBlocks);          // rows of a group whose exponents one register of the wave holds
@@ -123,7 +127,7 @@ __global__ __launch_bounds__((Grad<DT, TILE>::kThreads), 2) void weight_grad8_ke
     const bool role_x = wave >= G::kWaves / 2;               // stages the kept codes
     const int unit = role_x ? t - G::kThreads / 2 : t;
     const int cg = unit % G::kGroups, kg = unit / G::kGroups;
-    const int wm = TILE == 256 ? (wave & 1) * 128 : (wave & 1) * 64, wn = (wave >> 1) * 64;
+    const int wm = (wave & 1) * (TILE / 2), wn = (wave >> 1) * (TILE / 4);
     const bool sums = db && i0 == 0;
 
     f32x16 acc[G::MT][G::NT] = {};
@@ -272,40 +276,49 @@ __global__ __launch_bounds__((Grad<DT, TILE>::kThreads), 2) void weight_grad8_ke
         }
     };
 
-    // (every split has rows: rows_per_split and splits come from split_rows)
+    // Turn t multiplies step t out of one buffer and stages step t + 1 into the other (the first turn only stages); one copy of each part
+    // in the code: the kernel is small enough to be fetched in the time that a few steps take.  (Every split has rows.)
     fetch(r_begin);
-    stage(lds, r_begin);
-    if (r_begin + BK < r_end) fetch(r_begin + BK);
-    __syncthreads();
-    int cur = 0;
-    for (int64_t r0 = r_begin; r0 < r_end; r0 += BK, cur ^= 1) {
+    int cur = 1;
+    for (int64_t r0 = r_begin - BK; r0 < r_end; r0 += BK, cur ^= 1) {
         uint16_t *const here = lds + cur * G::kBuffer, *const next = lds + (cur ^ 1) * G::kBuffer;
         const bool more = r0 + BK < r_end, after = r0 + 2 * BK < r_end;
         if (!role_x) {
             if (more) stage(next, r0 + BK);
             if (after) fetch(r0 + 2 * BK);
-            multiply(here);
-        } else {
-            multiply(here);
+        }
+        if (r0 >= r_begin) multiply(here);
+        if (role_x) {
             if (more) stage(next, r0 + BK);
             if (after) fetch(r0 + 2 * BK);
         }
         __syncthreads();
     }
 
-    // C of the 32x32 instruction: column lane & 31, row (i & 3) + 8 (i >> 2) + 4 (lane >> 5)
+    // C of the 32x32 instruction: column lane & 31, row (i & 3) + 8 (i >> 2) + 4 (lane >> 5).  One run of stores for each place and type:
+    // (a choice for every element was half of the kernel's code and, cold, a fifth of its time at 12544 rows of 256)
+    auto write = [&](auto type, void *to) {
+        constexpr int OT = decltype(type)::value;
 #pragma unroll
-    for (int m = 0; m < G::MT; ++m)
+        for (int n = 0; n < G::NT; ++n) {
+            const int c = i0 + wn + n * 32 + (lane & 31);
+            if (c < in_f) {
 #pragma unroll
-        for (int n = 0; n < G::NT; ++n)
+                for (int m = 0; m < G::MT; ++m) {
+                    const int o = o0 + wm + m * 32 + 4 * (lane >> 5);
+                    char *p = (char *)to + ((int64_t)o * in_f + c) * (OT == SN_F32 ? 4 : 2);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int o = o0 + wm + m * 32 + (i & 3) + 8 * (i >> 2) + 4 * (lane >> 5), c = i0 + wn + n * 32 + (lane & 31);
-                if (o < out_f && c < in_f) {
-                    if (part_w) part_w[((int64_t)split * out_f + o) * in_f + c] = acc[m][n][i];
-                    else store_any(dw, out_dtype, (int64_t)o * in_f + c, acc[m][n][i]);
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = (i & 3) + 8 * (i >> 2);
+                        if (!SMALL || o + r < out_f) store_one<OT>(p + (int64_t)r * in_f * (OT == SN_F32 ? 4 : 2), 0, acc[m][n][i]);
+                    }
                 }
             }
+        }
+    };
+    if (part_w || out_dtype == SN_F32) write(Type<SN_F32>(), part_w ? (void *)(part_w + (int64_t)split * out_f * in_f) : dw);
+    else if (out_dtype == SN_BF16) write(Type<SN_BF16>(), dw);
+    else write(Type<SN_F16>(), dw);
     if (sums) {                                              // (the last turn ended with a barrier: LDS is free)
         float *red = reinterpret_cast<float *>(lds);         // [BK / 8 row groups][TILE columns]
         if (!role_x) {
@@ -440,7 +453,8 @@ extern "C" int sn_checkpoint8_restore(const void *codes, const void *exps, int64
                dtype);
     if (rows == 0) return SN_OK;
     SN_REQUIRE(out && codes && exps, SN_ERR_BAD_ARG, "sn_checkpoint8_restore: NULL pointer");
-    const dim3 grid(pack_blocks(rows * (((int64_t)n + 7) / 8))), block(kPackThreads);
+    const int ev = dtype == SN_F32 ? 4 : 8;
+    const dim3 grid(pack_blocks(rows * (((int64_t)n + ev - 1) / ev))), block(kPackThreads);
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == SN_F32) hipLaunchKernelGGL(restore8_kernel<SN_F32>, grid, block, 0, st, (const uint8_t *)codes, (const uint8_t *)exps, rows, n, out);
     else if (dtype == SN_BF16) hipLaunchKernelGGL(restore8_kernel<SN_BF16>, grid, block, 0, st, (const uint8_t *)codes, (const uint8_t *)exps, rows, n, out);
