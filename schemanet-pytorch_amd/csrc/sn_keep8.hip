@@ -287,7 +287,12 @@ __global__ __launch_bounds__((Grad<DT, TILE>::kThreads), 2) void weight_grad8_ke
             if (more) stage(next, r0 + BK);
             if (after) fetch(r0 + 2 * BK);
         }
-        if (r0 >= r_begin) multiply(here);
+        if (r0 >= r_begin) {
+            if (role_x) __builtin_amdgcn_s_setprio(2);
+            else __builtin_amdgcn_s_setprio(1);
+            multiply(here);
+            __builtin_amdgcn_s_setprio(0);
+        }
         if (role_x) {
             if (more) stage(next, r0 + BK);
             if (after) fetch(r0 + 2 * BK);
