@@ -200,6 +200,14 @@ __device__ __forceinline__ bool row_counts(const sn_block_norms_args &a, int64_t
     return (int)(row - g * a.rows_per_graph) < a.n_valid[g];
 }
 
+// the first row from r on, in steps of turn, that counts (or one behind the last)
+__device__ __forceinline__ int64_t next_row(const sn_block_norms_args &a, int64_t r, int64_t turn)
+{
+    if (a.n_valid)
+        while (r < a.rows && !row_counts(a, r)) r += turn;
+    return r;
+}
+
 struct NormStats { float mean, rstd; };
 
 // mean and 1 / deviation of a row; elements beyond E do not count (they are zeros)
@@ -227,10 +235,11 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
     return s;
 }
 
-// MODE: 0 = the parts of the call are looked up at run time; 1 = everything is there (2: but the gate), every row counts, nothing is
-// kept in 8 bits.  The branches of mode 0 make the compiler wait for all loads and stores in flight where it needs the oldest row,
-// the straight line of the others does not (rows of 4096 bf16, backward: 760 us for 32768 rows in mode 0, MODE_BWD_US in mode 1).
-template <int DT, int EV, int CH, bool MULTI, int MODE>
+// MODE: 0 = the parts of the call are looked up at run time; 1 = everything is there (2: but the gate).  The branches of mode 0 make the
+// compiler wait for all loads and stores in flight where it needs the oldest row, the straight line of the others does not
+// (backward of 32768 rows of 4096 bf16: 760 us in mode 0, 427 in mode 1).  For the same reason rows that do not count are passed
+// over by scalar arithmetic, and get their zeros in a loop of their own.
+template <int DT, int EV, int CH, bool MULTI, int MODE, bool KEEP>
 __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block_norms_args a)
 {
     using L = Layout<DT, EV, CH, MULTI>;
@@ -245,25 +254,24 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block
     const int t = MULTI ? threadIdx.x : threadIdx.x & 63;
     const int E = a.width, step = (MULTI ? (int)blockDim.x : 64) * EV, col = t * EV, npad = (E + 31) & ~31;
     const float inv_e = 1.0f / (float)E;
-    const bool gated = ALL ? MODE == 1 : a.gate != nullptr, post = ALL || a.has_post, pre = ALL || a.has_pre, keep = !ALL && a.x_codes;
+    const bool gated = ALL ? MODE == 1 : a.gate != nullptr, post = ALL || a.has_post, pre = ALL || a.has_pre;
     const bool tail = __any(tail_shift<EV>(col + (CH - 1) * step, E) > 0);
     const int64_t turn = (int64_t)gridDim.x * L::kRows;
 
-    struct Slot { Ahead<DT, EV, CH> x, f, z; bool live; };
+    struct Slot { Ahead<DT, EV, CH> x, f, z; };
     auto issue = [&](Slot &s, int64_t row) {
-        if constexpr (ALL) row = row < a.rows ? row : a.rows - 1;
-        else {
-            s.live = row_counts(a, row);
-            if (!s.live) return;
-        }
         issue_cols<DT, EV, CH, L::kTiny>(s.x, a.x, row, a.x_stride, col, step, E);
         issue_cols<DT, EV, CH, L::kTiny>(s.f, a.branch, row, a.branch_stride, col, step, E);
         if (gated) issue_cols<DT, EV, CH, L::kTiny>(s.z, a.gate, row, a.gate_stride, col, step, E);
     };
     const int64_t start = (int64_t)blockIdx.x * L::kRows + group;
     Slot s0, s1;
-    issue(s0, start);
-    if constexpr (L::kAheadForward == 2) issue(s1, start + turn);
+    int64_t ra = next_row(a, start, turn), rb = a.rows;
+    if (ra < a.rows) {
+        issue(s0, ra);
+        rb = next_row(a, ra + turn, turn);
+        if constexpr (L::kAheadForward == 2) issue(s1, rb < a.rows ? rb : ra);
+    }
     Row<EV, CH> w1, b1, sc, w2, b2;
     load_param<EV, CH>(sc, a.scale, a.param_dtype, col, step, E, 1.0f);
     load_param<EV, CH>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
@@ -271,19 +279,14 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block
     load_param<EV, CH>(w2, pre ? a.pre_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
     load_param<EV, CH>(b2, pre ? a.pre_bias : nullptr, a.param_dtype, col, step, E, 0.0f);
 
-    auto work = [&](Slot &s, int64_t row) {
-        if (!ALL && !s.live) {                               // the same for every wave of the row
-            issue(s, row + L::kAheadForward * turn);
-            zero_cols<DT, EV, CH>(a.y, row, col, step, E);
-            if (pre) zero_cols<DT, EV, CH>(a.h, row, col, step, E);
-            return;
-        }
+    // row r out of s, which then takes row `after` (behind the last: r again, never used)
+    auto work = [&](Slot &s, int64_t row, int64_t after) {
         Row<EV, CH> x, f, z;
         take_cols<DT, EV, CH>(x, s.x, col, step, E, tail);
         take_cols<DT, EV, CH>(f, s.f, col, step, E, tail);
         if (gated) take_cols<DT, EV, CH>(z, s.z, col, step, E, tail);
-        issue(s, row + L::kAheadForward * turn);
-        if (keep) {
+        issue(s, after < a.rows ? after : row);
+        if constexpr (KEEP) {
             store_checkpoint<EV, CH>(a.x_codes, a.x_exps, row, col, step, npad, x);
             store_checkpoint<EV, CH>(a.branch_codes, a.branch_exps, row, col, step, npad, f);
             if (gated) store_checkpoint<EV, CH>(a.gate_codes, a.gate_exps, row, col, step, npad, z);
@@ -311,11 +314,26 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block
         }
         if (a.stats && t == 0) *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(n1.mean, n1.rstd, n2.mean, n2.rstd);
     };
-    for (int64_t row = start; row < a.rows; row += L::kAheadForward * turn) {
-        work(s0, row);
+    while (ra < a.rows) {
         if constexpr (L::kAheadForward == 2) {
-            if (row + turn >= a.rows) break;
-            work(s1, row + turn);
+            const int64_t rc = next_row(a, rb + turn, turn);
+            work(s0, ra, rc);
+            if (rb >= a.rows) break;
+            const int64_t rd = next_row(a, rc + turn, turn);
+            work(s1, rb, rd);
+            ra = rc;
+            rb = rd;
+        } else {
+            work(s0, ra, rb);
+            ra = rb;
+            rb = next_row(a, rb + turn, turn);
+        }
+    }
+    if (a.n_valid) {
+        for (int64_t row = start; row < a.rows; row += turn) {
+            if (row_counts(a, row)) continue;
+            zero_cols<DT, EV, CH>(a.y, row, col, step, E);
+            if (pre) zero_cols<DT, EV, CH>(a.h, row, col, step, E);
         }
     }
 }
@@ -344,14 +362,8 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
         Ahead<DT, EV, CH> x, f, z, dy, dh;
         AheadKept<EV, CH> kx, kf, kz;
         float4 st;
-        bool live;
     };
     auto issue = [&](Slot &s, int64_t row) {
-        if constexpr (ALL) row = row < a.rows ? row : a.rows - 1;
-        else {
-            s.live = row_counts(a, row);
-            if (!s.live) return;
-        }
         if constexpr (KEPT) {
             issue_kept<EV, CH>(s.kx, a.x_codes, a.x_exps, row, col, step, npad);
             issue_kept<EV, CH>(s.kf, a.branch_codes, a.branch_exps, row, col, step, npad);
@@ -367,8 +379,12 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
     };
     const int64_t start = (int64_t)blockIdx.x * L::kRows + group;
     Slot s0, s1;
-    issue(s0, start);
-    if constexpr (L::kAheadBackward == 2) issue(s1, start + turn);
+    int64_t ra = next_row(a, start, turn), rb = a.rows;
+    if (ra < a.rows) {
+        issue(s0, ra);
+        rb = next_row(a, ra + turn, turn);
+        if constexpr (L::kAheadBackward == 2) issue(s1, rb < a.rows ? rb : ra);
+    }
     Row<EV, CH> w1, b1, sc, w2;
     load_param<EV, CH>(sc, a.scale, a.param_dtype, col, step, E, 1.0f);
     load_param<EV, CH>(w1, post ? a.post_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
@@ -376,14 +392,8 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
     load_param<EV, CH>(w2, has_dh ? a.pre_weight : nullptr, a.param_dtype, col, step, E, 1.0f);
     Row<EV, CH> sum[kVectors] = {};
 
-    auto work = [&](Slot &s, int64_t row) {
-        if (!ALL && !s.live) {
-            issue(s, row + L::kAheadBackward * turn);
-            if (a.dx) zero_cols<DT, EV, CH>(a.dx, row, col, step, E);
-            if (a.dbranch) zero_cols<DT, EV, CH>(a.dbranch, row, col, step, E);
-            if (a.dgate) zero_cols<DT, EV, CH>(a.dgate, row, col, step, E);
-            return;
-        }
+    // row r out of s, which then takes row `after` (behind the last: r again, never used)
+    auto work = [&](Slot &s, int64_t row, int64_t after) {
         Row<EV, CH> x, f, z, u = {}, d;
         if constexpr (KEPT) {
             take_kept<EV, CH>(x, s.kx, col, step, npad);
@@ -397,7 +407,7 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
         if (has_dy) take_cols<DT, EV, CH>(u, s.dy, col, step, E, tail);
         if (has_dh) take_cols<DT, EV, CH>(d, s.dh, col, step, E, tail);
         const float4 st = s.st;
-        issue(s, row + L::kAheadBackward * turn);
+        issue(s, after < a.rows ? after : row);
         // f -> unit values of the post norm, z -> sigmoid, x -> unit values of y.  Columns beyond E hold whatever the statistics make of
         // zeros: every use multiplies it by a weight or a gradient that is zero there, and no store takes it.
 #pragma unroll
@@ -462,11 +472,27 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
         }
         if (ALL || a.dbranch) store_cols<DT, EV, CH>(a.dbranch, row, col, step, E, d);
     };
-    for (int64_t row = start; row < a.rows; row += L::kAheadBackward * turn) {
-        work(s0, row);
+    while (ra < a.rows) {
         if constexpr (L::kAheadBackward == 2) {
-            if (row + turn >= a.rows) break;
-            work(s1, row + turn);
+            const int64_t rc = next_row(a, rb + turn, turn);
+            work(s0, ra, rc);
+            if (rb >= a.rows) break;
+            const int64_t rd = next_row(a, rc + turn, turn);
+            work(s1, rb, rd);
+            ra = rc;
+            rb = rd;
+        } else {
+            work(s0, ra, rb);
+            ra = rb;
+            rb = next_row(a, rb + turn, turn);
+        }
+    }
+    if (a.n_valid) {
+        for (int64_t row = start; row < a.rows; row += turn) {
+            if (row_counts(a, row)) continue;
+            if (a.dx) zero_cols<DT, EV, CH>(a.dx, row, col, step, E);
+            if (a.dbranch) zero_cols<DT, EV, CH>(a.dbranch, row, col, step, E);
+            if (a.dgate) zero_cols<DT, EV, CH>(a.dgate, row, col, step, E);
         }
     }
     if (partial) {
@@ -548,8 +574,11 @@ template <int DT, int EV, int CH, bool MULTI> int launch_forward(const sn_block_
 {
     using L = Layout<DT, EV, CH, MULTI>;
     const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = MULTI ? 256 * (16 / waves_for(a.width)) : 2048, each = (turns + most - 1) / most;
-    const bool all = a.has_post && a.has_pre && !a.n_valid && !a.x_codes;
-    const auto kernel = !all ? norms_forward_kernel<DT, EV, CH, MULTI, 0> : a.gate ? norms_forward_kernel<DT, EV, CH, MULTI, 1> : norms_forward_kernel<DT, EV, CH, MULTI, 2>;
+    const bool all = a.has_post && a.has_pre;
+    const auto kernel = a.x_codes ? (!all ? norms_forward_kernel<DT, EV, CH, MULTI, 0, true> : a.gate ? norms_forward_kernel<DT, EV, CH, MULTI, 1, true>
+                                                                                                      : norms_forward_kernel<DT, EV, CH, MULTI, 2, true>)
+                                  : (!all ? norms_forward_kernel<DT, EV, CH, MULTI, 0, false> : a.gate ? norms_forward_kernel<DT, EV, CH, MULTI, 1, false>
+                                                                                                       : norms_forward_kernel<DT, EV, CH, MULTI, 2, false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)((turns + each - 1) / each)), dim3(MULTI ? waves_for(a.width) * 64 : 256), 0, st, a);
     SN_CHECK_LAUNCH("sn_block_norms_forward");
     return SN_OK;
@@ -562,7 +591,7 @@ template <int DT, int EV, int CH, bool MULTI> int launch_backward(const sn_block
     for (int k = 0; k < kVectors; ++k) columns |= out.p[k] != nullptr;
     float *partial = columns ? (float *)a.workspace : nullptr;
     const bool gate = a.x_codes ? a.gate_codes != nullptr : a.gate != nullptr;
-    const bool all = a.has_post && a.has_pre && !a.n_valid && a.dy && a.dh && a.dx && a.dbranch && (!gate || a.dgate);
+    const bool all = a.has_post && a.has_pre && a.dy && a.dh && a.dx && a.dbranch && (!gate || a.dgate);
     const auto kernel = a.x_codes ? (!all ? norms_backward_kernel<DT, EV, CH, MULTI, 0, true> : gate ? norms_backward_kernel<DT, EV, CH, MULTI, 1, true>
                                                                                                       : norms_backward_kernel<DT, EV, CH, MULTI, 2, true>)
                                   : (!all ? norms_backward_kernel<DT, EV, CH, MULTI, 0, false> : gate ? norms_backward_kernel<DT, EV, CH, MULTI, 1, false>
