@@ -57,7 +57,8 @@ template <int DT> __device__ __forceinline__ float sigmoid(float z)
     float e = __builtin_amdgcn_exp2f(t);
     if constexpr (DT == SN_F32) {
         const float lo = fmaf(-z, L, -t) - z * Llo;
-        e = t < 126.0f ? fmaf(e, lo * ln2, e) : e;           // (beyond it e may be infinite, and the sigmoid is under 2^-126)
+        // (beyond 2^126 e may be infinite and the sigmoid is under 2^-126; under 2^-126 e no longer shows in 1 + e; an infinite z has no lo)
+        e = fabsf(t) < 126.0f ? fmaf(e, lo * ln2, e) : e;
     }
     return __builtin_amdgcn_rcpf(1.0f + e);
 }

@@ -328,6 +328,33 @@ def test_norms_extreme_rows(ops):
     assert torch.isnan(h[2]).all() and torch.isfinite(h[[0, 1, 4, 5]]).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_norms_closed_and_open_gates(ops, dtype):
+    """gates at the ends of their type, infinities among them: sigmoid 0 or 1 exactly, a gradient of 0 for the gate"""
+    t = norm_inputs(gen(17), (4, 300), dtype)
+    t["gate"][0], t["gate"][1] = float("inf"), float("-inf")
+    t["gate"][2], t["gate"][3] = 88.5, -200.0
+    x, z = t["x"].clone().requires_grad_(), t["gate"].clone().requires_grad_()
+    y, h = ops.gated_residual_norms(x, t["branch"], gate=z, scale=t["scale"], post=t["post"], pre=t["pre"])
+    want = Norms64(d64(t["x"]), d64(t["branch"]), d64(t["gate"]), d64(t["scale"]), tuple(map(d64, t["post"])), tuple(map(d64, t["pre"])), "layer", 1e-5)
+    check(y, want.y, HALF[dtype] * want.y.abs() + K_ROW * U * want.y_mag * 2 + TINY[dtype], "y")
+    check(h, want.h, HALF[dtype] * want.h.abs() + K_ROW * U * want.h_mag * 2 + TINY[dtype], "h")
+    assert torch.equal(y[1], t["x"][1])
+    dz, dx = torch.autograd.grad((y.float().sum() + h.float().sum()), [z, x])
+    assert not dz[:2].any() and torch.isfinite(dx).all() and torch.isfinite(dz).all()
+
+
+@pytest.mark.parametrize("n_valid", [[0, 0, 0], [-1, 7, 100], [3, 0, 4]])
+def test_norms_extents_outside_the_graph(ops, n_valid):
+    """no vertex at all, and extents beyond the padded length (= every vertex) or below zero (= none)"""
+    t = norm_inputs(gen(18), (3, 5, 70), F32)
+    nv = torch.tensor(n_valid, dtype=torch.int32, device=DEV)
+    check_norms(ops, t, "layer", F32, n_valid=nv.clamp(0, 5))
+    y, h = ops.gated_residual_norms(t["x"], t["branch"], gate=t["gate"], pre=t["pre"], n_valid=nv)
+    y2, h2 = ops.gated_residual_norms(t["x"], t["branch"], gate=t["gate"], pre=t["pre"], n_valid=nv.clamp(0, 5))
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
 @pytest.mark.parametrize("keep8", [False, True])
 def test_norms_gradient_against_differences(ops, keep8):
     """the derivative along a direction from central differences of the float64 definition; with 8-bit checkpoints the inputs are such
