@@ -14,7 +14,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kPackThreads = 256;
 
-// HBM bound: one read of x, 1 + 1/32 bytes written per element; a lane holds 8 features, four lanes a block
+// HBM bound: one read of x, 1 + 1/32 bytes written per element; a lane holds 8 features, four lanes a block.  32768 rows of 2048, bf16:
+// 36 us, 5.6 TB/s
 template <int DT>
 __global__ __launch_bounds__(kPackThreads) void checkpoint8_kernel(const void *x, int64_t rows, int n, int64_t stride, uint8_t *codes, uint8_t *exps)
 {
@@ -63,7 +64,12 @@ __global__ __launch_bounds__(kPackThreads) void restore8_kernel(const uint8_t *c
 // staging thread takes 8 rows of UC columns, turns them in registers (the bf16 conversion pairs two ROWS into a word) and
 // writes 8 consecutive rows of one column to LDS, as the matrix instruction wants them.  Half of the waves stage dY, the other
 // half the kept codes; two LDS buffers, one barrier a step; the dY waves stage before their products and the code waves after
-// them, so that on every SIMD the vector work of one wave runs under the matrix instructions of the other.
+// them, so that on every SIMD the vector work of one wave runs under the matrix instructions of the other; priorities keep that
+// order (code waves multiply first: 1061 -> 1040 us at the size below).
+// Bound: the matrix pipe with the vector work beside it (64 codes are 160 vector instructions a step, a third of the issue slots).
+// 32768 rows of 2048 -> 8192, bf16: 1040 us, 1057 TFLOP/s; the library's product of the same operands, both in bf16, takes 937 us.
+// fp32 gradients (three products): 32768 rows of 2048 -> 2048 698 us, 394 TFLOP/s (1.18 PFLOP/s of matrix work), fp16 485 us.
+// Small sizes are bound by a few steps' latency: 12544 rows of 256 -> 256, fp32: 14 us and 5 us for the joining of 49 splits.
 typedef uint32_t u32;
 
 template <int V> struct Type { static constexpr int value = V; };

@@ -2,14 +2,15 @@
 //     d_j = x_j - max x;  s = sum exp(d);  t = sum exp(d) d;   log p_j = d_j - log s;   H = log s - t / s
 //     grad_j = g (delta_jt - p_j) - g_H p_j (log p_j + H)
 // Bound: HBM - forward reads the logits once (running max, s and t per lane, joined at the end; the top list is kept beside
-// them), backward reads them once and writes the gradient.  A row belongs to one wave (up to kWaveRow entries), to the four
+// them), backward reads them once and writes the gradient.  A row belongs to one wave, to the four
 // waves of a workgroup, or - few rows - to up to 64 workgroups whose partial results a second launch joins.
+// Measured (the card copies at 5.13 TB/s): 4096 rows of 32769, bf16: forward and backward pass 82 + 85 us of kernels (805 MB, 4.8 TB/s);
+// 16 rows of 131072, bf16, 20 alternatives: 10.6 + 5.8 us; one row of 1000, fp32, 5 alternatives: 5.3 us (3.4 without them): latency.
 //
-// Top list: a wave keeps its k best (value, index) sorted across its lanes, lane j the j-th.  The first 1024 elements fill it through a
-// bound that the lanes' maxima give (fill_list); after that a group of elements is looked at again only if one of them beats
-// the k-th, and an insertion is one ballot (its place) and one shift by a lane.  Order: larger value first, lower index among
-// equals.  Lists are joined in pairs: an element's place in the join is its own plus the number of the partner's that come
-// before it (binary search).
+// Top list: a wave keeps its k best (value, index) sorted across its lanes, lane j the j-th.  A group of 1024 elements is looked at again
+// only if one of them beats the k-th: a few candidates are inserted one by one (one ballot for the place, one shift by a lane),
+// more are gathered, sorted and merged at once (absorb).  Order: larger value first, lower index among equals, as one 64-bit
+// number.
 #include "sn_typed.h"
 
 namespace {
@@ -17,7 +18,6 @@ namespace {
 using namespace sn;
 
 constexpr int kScoreThreads = 256, kScoreWaves = 4;
-constexpr int64_t kWaveRow = 2048;       // entries of a row that one wave takes
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 // stands for any distance beyond it where it is multiplied by exp(d): exp(-10^4) = 0 in fp32, and 0 times an infinite d must stay 0
@@ -550,10 +550,16 @@ __global__ __launch_bounds__(kScoreThreads) void scores_backward_kernel(ScoreGra
     }
 }
 
+// One wave a row: short rows, and longer ones where there are waves enough (us, wave against workgroup, bf16, without | with 5
+// alternatives: 256 x 2048 4.0, 3.8 | 8.4, 8.1; 256 x 4096 5.0, 3.9 | 13.2, 8.1; 1024 x 4096 5.2, 5.6 | 13.4, 13.1; 2048 x 8192 10.3,
+// 10.6 | 23.7, 28.0; 4096 x 16384 26.5, 28.5 | 50.2, 67.8; 4096 x 32769 49.0, 47.2 | 76.0, 99.8)
+bool wave_a_row(int64_t rows, int64_t n) { return n <= 2048 || (rows >= 2048 && n <= 16384); }
+// Workgroups a row: one up to 8192 entries (one row of 8192: 3.8 us, in two parts and joined 6.0), else four for each compute unit of
+// 4096 entries or more (16 x 131072, bf16, 20 alternatives: parts of 4096 15.5 us, 8192 16.2, 16384 21.0, 2048 17.9)
 int splits_for(int64_t rows, int64_t n)
 {
-    if (n <= kWaveRow || rows <= 0) return 1;
-    int64_t s = 1024 / rows;                                 // four workgroups for each compute unit
+    if (n <= 8192 || rows <= 0 || wave_a_row(rows, n)) return 1;
+    int64_t s = 1024 / rows;
     const int64_t most = (n + 4095) / 4096;
     s = s > most ? most : s;
     s = s > kMaxSplits ? kMaxSplits : s;
@@ -562,7 +568,7 @@ int splits_for(int64_t rows, int64_t n)
 
 template <int DT, bool TOP> int launch_scores(ScoreArgs &a, hipStream_t st)
 {
-    if (a.n <= kWaveRow) {
+    if (wave_a_row(a.rows, a.n)) {
         const int64_t blocks = (a.rows + kScoreWaves - 1) / kScoreWaves;
         hipLaunchKernelGGL((scores_wave_kernel<DT, TOP>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(kScoreThreads), 0, st, a);
         SN_CHECK_LAUNCH("sn_label_log_probs");
@@ -624,6 +630,7 @@ extern "C" int sn_label_log_probs_backward(const void *logits, int dtype, int64_
     if (rows == 0) return SN_OK;
     SN_REQUIRE(stats && grad && (g_log_probs || g_entropy), SN_ERR_BAD_ARG, "sn_label_log_probs_backward: NULL pointer");
     const ScoreGradArgs a = {logits, rows, n, row_stride, target, ignore_index, stats, g_log_probs, g_entropy, grad};
+    // (pieces of a row, us for 4096 x 32768 bf16: 2048 118, 4096 104, 8192 99, 16384 102, 32768 107)
     const int64_t per = 8192, pieces = (n + per - 1) / per;
     SN_REQUIRE(rows * pieces < (1ll << 31), SN_ERR_UNSUPPORTED, "sn_label_log_probs_backward: too large");
     const dim3 grid((unsigned)(rows * pieces)), block(kScoreThreads);

@@ -438,7 +438,8 @@ def check_scores(ops, x, target, topk=0, grads=True, ignore=-100, seed=0):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("rows,n", [(1, 1), (3, 2), (5, 7), (4, 100), (9, 512), (3, 1000), (2, 2048), (3, 2049), (2, 5001), (5, 32769), (1, 131072), (700, 4100)])
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 2), (5, 7), (4, 100), (9, 512), (3, 1000), (2, 2048), (3, 2049), (2, 5001), (5, 32769), (1, 131072), (700, 4100), (3, 8192), (3, 8193), (2048, 2100), (2100, 5001),
+                                     (2047, 16385)])
 def test_scores_sizes(ops, dtype, rows, n):
     g = gen(rows * 7 + n)
     x = rand(g, rows, n, dtype=dtype, std=3.0)
