@@ -242,8 +242,8 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
 
 // MODE: 0 = the parts of the call are looked up at run time; 1 = everything is there (2: but the gate).  The branches of mode 0 make the
 // compiler wait for all loads and stores in flight where it needs the oldest row, the straight line of the others does not
-// (backward of 32768 rows of 4096 bf16 with the same look-ahead of one row: 761 us looked up, 427 straight and two ahead).  For the same reason rows that do not count are passed
-// over by scalar arithmetic, and get their zeros in a loop of their own.
+// (backward of 32768 rows of 4096 bf16: 761 us looked up and one row ahead, 427 straight and two ahead).  For the same reason rows that
+// do not count are passed over by scalar arithmetic, and get their zeros in a loop of their own.
 template <int DT, int EV, int CH, bool MULTI, int MODE, bool KEEP>
 __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block_norms_args a)
 {
@@ -551,14 +551,21 @@ __global__ __launch_bounds__(1024) void norms_columns_kernel(const float *partia
     if (lane == 0 && c < E) store_any(out.p[k], dtype, c, s);
 }
 
-// lanes of a row: 8 elements a lane up to 4096 columns (16 waves with five column sums each would spill); 4 a lane under 257 columns
+// Waves of a row: 8 elements a lane up to 4096 columns (16 waves with five column sums each would spill).  Up to 256 columns a lane
+// takes 4: all lanes work and more waves are resident (bf16, 200000 rows forward / backward: 256 columns 108 / 212 us, with 8 a lane
+// 152 / 230; 128 columns 104 / 193, with 8 a lane 152 / 227).
 int waves_for(int E) { return (E + 511) / 512; }
 int rows_per_block(int E) { return waves_for(E) > 1 ? 1 : 4; }
 int backward_blocks(int64_t rows, int E)
 {
     const int64_t turns = (rows + rows_per_block(E) - 1) / rows_per_block(E);
-    // as many workgroups as are resident with the registers of the backward kernel: two waves a SIMD (one wave a row of up to 256: four)
-    const int64_t most = waves_for(E) == 1 ? 1024 : 256 * (8 / waves_for(E)), each = (turns + most - 1) / most;
+    // Workgroups: enough waves to cover the loads, no more: each further one loads the parameters again, writes a line of column sums,
+    // and has fewer rows to look ahead over.  Four workgroups of four waves a compute unit, about six waves of the wider rows (measured
+    // with 1, 2, 3, 4, 6, 8 workgroups a compute unit: bf16 131072 x 1024 756 493 411 438 478 497 us; 65536 x 2048 413 447 500 486 488
+    // 556; 32768 x 4096 420 434 465 465 500 541; fp32 32768 x 2048 405 430 446 436 462 454; one wave, fp32 200000 x 256 650 397 320 301
+    // 355 322; bf16 200000 x 512 330 326 336 341 346 350).
+    const int W = waves_for(E);
+    const int64_t most = 256 * (W == 1 ? 4 : W > 6 ? 1 : 6 / W), each = (turns + most - 1) / most;
     return (int)((turns + each - 1) / each);                 // (the same number of turns for all but the last)
 }
 
@@ -578,7 +585,11 @@ int check_args(const sn_block_norms_args *a, const char *who)
 template <int DT, int EV, int CH, bool MULTI> int launch_forward(const sn_block_norms_args &a, hipStream_t st)
 {
     using L = Layout<DT, EV, CH, MULTI>;
-    const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = MULTI ? 256 * (16 / waves_for(a.width)) : 2048, each = (turns + most - 1) / most;
+    // Workgroups a compute unit: eight of four waves, eight waves of the wider rows (measured with 1, 2, 3, 4, 8, 16 workgroups: bf16
+    // 131072 x 1024 750 453 311 263 269 280 us; 65536 x 2048 394 275 288 287 286 308; 32768 x 4096 254 271 280 265 266 261; one wave,
+    // fp32 103424 x 256 with 4, 8, 16, 32: 100 109 108 116, bf16 200000 x 256 with 2, 4, 8, 16: 134 106 109 103).
+    const int W = waves_for(a.width);
+    const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = 256 * (MULTI ? (8 + W - 1) / W : 8), each = (turns + most - 1) / most;
     const bool all = a.has_post && a.has_pre;
     const auto kernel = a.x_codes ? (!all ? norms_forward_kernel<DT, EV, CH, MULTI, 0, true> : a.gate ? norms_forward_kernel<DT, EV, CH, MULTI, 1, true>
                                                                                                       : norms_forward_kernel<DT, EV, CH, MULTI, 2, true>)
