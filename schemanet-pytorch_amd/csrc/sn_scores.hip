@@ -165,18 +165,18 @@ template <int N> __device__ __forceinline__ int count_from(const float (&x)[N], 
 }
 
 // The list's new state after N elements a lane (x, their indexes index(u), all behind those it has seen).  Candidates are the elements from
-// a bound on: the k-th largest of the 64 lanes' maxima for an empty list (at least k elements reach it), else what lies above the
-// list's last entry.  More than 64 of them: the bound is raised by bisection over the values' bits to the largest that k elements
+// a bound on: what lies above the last entry of a full list; until it is full, the k-th largest of the 64 lanes' maxima (at least k
+// elements reach it) or, with fewer lanes above -inf, all elements there.  More than 64 of them: the bound is raised by bisection over the values' bits to the largest that k elements
 // reach; where that still leaves more than 64 - equal values - those above it and the first of the equal ones by index (EV elements of
 // a lane lie behind one another).  The candidates are gathered, sorted and merged with the list (larger of entry i and entry
 // 63 - i of the other, then the last merge of the sort).  room: 64 entries of LDS of this wave
 template <int EV, int N, class Index> __device__ __forceinline__ void absorb(TopList &top, const float (&x)[N], float lane_max, Index index, int k, Key *room)
 {
     const int lane = threadIdx.x & 63;
-    const bool empty = top.last == kNone;
+    const bool full = top.last != kNone, empty = lane_key(top.key, 0) == kNone;
     float b = lane_max;
     uint32_t low;
-    if (empty) {
+    if (!full) {
         wave_sort(b);
         low = ordered(fmaxf(SN_READLANE_F32(b, k - 1), kLowest));                // (never an entry at -inf)
     } else {

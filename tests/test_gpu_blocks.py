@@ -485,6 +485,20 @@ def test_scores_masks(ops, dtype, n):
     assert got.top_ids[2].tolist() == [0, 1, 2] and got.top_ids[1].tolist() == [n - 1, 0, 1] and float(got.log_probs[6]) == 0.0
 
 
+@pytest.mark.parametrize("topk", [1, 7, 64])
+@pytest.mark.parametrize("n", [300, 2000, 7000, 16000, 60000])
+def test_scores_few_entries_left(ops, n, topk):
+    """constrained answers: a few entries far apart, more and fewer of them than alternatives"""
+    g = gen(n + topk)
+    rows = 12
+    x = torch.full((rows, n), float("-inf"))
+    for r in range(rows):
+        left = torch.randperm(n, generator=g)[:[1, 2, 3, 5, 6, 7, 8, 9, 40, 63, 64, 100][r]]
+        x[r, left] = torch.randn(len(left), generator=g)
+    target = x.argmax(-1)
+    check_scores(ops, x.to(DEV), target.to(DEV), topk=topk)
+
+
 @pytest.mark.parametrize("n", [40, 5000, 40000])
 def test_scores_not_a_number(ops, n):
     g = gen(n)
