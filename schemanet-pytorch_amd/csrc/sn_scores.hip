@@ -520,8 +520,12 @@ __global__ __launch_bounds__(kScoreThreads) void scores_backward_kernel(ScoreGra
     const float g = used && a.g_lp ? a.g_lp[row] : 0.0f, gh = a.g_h ? a.g_h[row] : 0.0f;
     const char *src = (const char *)a.logits + (row * a.stride + c0) * SIZE;
     char *dst = (char *)a.grad + (row * a.n + c0) * SIZE;
-    const bool none = s == 0.0f;                             // a row without a distribution
     const bool wrong = used && (tg < 0 || tg >= a.n);
+    if (!wrong && (s == 0.0f || (g == 0.0f && gh == 0.0f))) {        // a row without a distribution, or without a part in the loss: not read
+        const float zeros[EV] = {};
+        for (int j = threadIdx.x * EV; j < n; j += kScoreThreads * EV) store_row<DT, EV>(dst, j, n, zeros);
+        return;
+    }
     const float ls = logf(s), inv = 1.0f / s;
     const int at = used && !wrong && tg >= c0 && tg < c0 + n ? (int)(tg - c0) : -1;
     for (int j = threadIdx.x * EV; j < n; j += kScoreThreads * EV) {
@@ -543,7 +547,6 @@ __global__ __launch_bounds__(kScoreThreads) void scores_backward_kernel(ScoreGra
             const float lg = fmaxf(d - ls, kFar);
             x[e] = -p * fmaf(gh, lg + h, g);
             if (j + e == at) x[e] += g;
-            if (none) x[e] = 0.0f;
             if (wrong) x[e] = __uint_as_float(0x7FC00000u);
         }
         store_row<DT, EV>(dst, j, n, x);
@@ -578,7 +581,7 @@ template <int DT, bool TOP> int launch_scores(ScoreArgs &a, hipStream_t st)
     SN_CHECK_LAUNCH("sn_label_log_probs");
     if (a.splits > 1) {
         const size_t lds = TOP ? (size_t)2 * a.splits * a.k * sizeof(Key) : 0;
-        const int rc = sn_ensure_dynamic_lds((const void *)scores_join_kernel<DT, TOP>, lds, "sn_label_log_probs");
+        const int rc = sn_ensure_dynamic_lds((const void *)scores_join_kernel<DT, TOP>, lds + sizeof(Select), "sn_label_log_probs");
         if (rc != SN_OK) return rc;
         hipLaunchKernelGGL((scores_join_kernel<DT, TOP>), dim3((unsigned)a.rows), dim3(kScoreThreads), lds, st, a);
         SN_CHECK_LAUNCH("sn_label_log_probs (join)");

@@ -84,12 +84,12 @@ class CEEntropyLoss(Loss):
             got = ops.label_log_probs(scores, label, ignore_index=self.ignore_index)
             log_probs, ent = got.log_probs, got.entropy
         else:
-            lp = torch.log_softmax(scores.float(), dim=-1)
-            log_probs = lp.gather(-1, label.masked_fill(~used, 0).unsqueeze(-1)).squeeze(-1) * used
+            lp = torch.log_softmax(scores.float().masked_fill(~used.unsqueeze(-1), 0.0), dim=-1)
+            log_probs = lp.gather(-1, label.masked_fill(~used, 0).unsqueeze(-1)).squeeze(-1).masked_fill(~used, 0.0)
             p = lp.exp()
             ent = -(p * lp.masked_fill(p == 0, 0.0)).sum(-1)
         count = used.sum()
-        return OrderedDict([("cls", -log_probs.sum() / count), ("entropy", (ent * used).sum() / count)])
+        return OrderedDict([("cls", -log_probs.sum() / count), ("entropy", ent.masked_fill(~used, 0.0).sum() / count)])
 
 
 class SchemaInferenceLoss(Loss):

@@ -499,6 +499,34 @@ def test_scores_few_entries_left(ops, n, topk):
     check_scores(ops, x.to(DEV), target.to(DEV), topk=topk)
 
 
+def test_scores_most_parts_with_most_alternatives(ops):
+    """rows so long that 64 workgroups share one"""
+    g = gen(3)
+    x = rand(g, 2, 300000, std=2.0)
+    check_scores(ops, x, x.argmin(-1), topk=64)
+    check_scores(ops, (x > 3).float(), x.argmin(-1), topk=64)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [9, 3000, 20000])
+def test_scores_rows_without_a_part_in_the_loss(ops, dtype, n):
+    """ignored rows, NaN or infinite as padding may be, get zeros; the others what they get alone"""
+    g = gen(n)
+    x = rand(g, 6, n, dtype=dtype, std=2.0)
+    x[1] = float("nan")
+    x[3] = float("inf")
+    x[4] = float("-inf")
+    target = torch.randint(0, n, (6,), generator=g).to(DEV)
+    target[[1, 3, 4]] = -100
+    used = target != -100
+    leaf, alone = x.clone().requires_grad_(), x[used].clone().requires_grad_()
+    got, part = ops.label_log_probs(leaf, target), ops.label_log_probs(alone, target[used])
+    grad, = torch.autograd.grad(got.log_probs.sum() + got.entropy.masked_fill(~used, 0.0).sum(), leaf)
+    want, = torch.autograd.grad(part.log_probs.sum() + part.entropy.sum(), alone)
+    assert not bool(grad[~used].any()) and torch.equal(grad[used], want)
+    assert torch.equal(got.log_probs[used], part.log_probs) and not bool(got.log_probs[~used].any())
+
+
 @pytest.mark.parametrize("n", [40, 5000, 40000])
 def test_scores_not_a_number(ops, n):
     g = gen(n)
