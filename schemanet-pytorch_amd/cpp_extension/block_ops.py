@@ -6,6 +6,7 @@ They take CUDA tensors in float32, bfloat16 or float16 with rows of any stride, 
 once; outputs are new contiguous tensors; nothing synchronises, all of them can be captured into a graph.  Under `torch.autocast`
 their floating-point inputs are cast to float32, like those of the other HIP-backed ops of this package.  Arguments that do not
 fit raise RuntimeError before anything is launched."""
+import math
 import struct
 from collections import namedtuple
 
@@ -120,10 +121,19 @@ class Checkpoint8:
     def nbytes(self):
         return self.codes.numel() + self.exps.numel()
 
+    def whole(self):
+        """do codes and exponents have the layout that `shape` asks for?  (the kernels read them by it)"""
+        n, codes, exps = self.shape[-1], self.codes, self.exps
+        rows, npad = math.prod(self.shape[:-1]), (n + 31) // 32 * 32
+        return (codes.dtype == torch.int8 and exps.dtype == torch.uint8 and codes.shape == (rows, npad) and exps.shape == (rows, npad // 32)
+                and codes.is_contiguous() and exps.is_contiguous())
+
     def restore(self, dtype=None):
         """the kept values, [..., n] in `dtype` (default: the type of the activation; bfloat16 and float32 hold them exactly)"""
         dtype = dtype or self.dtype
         _need(dtype in _TYPES, "checkpoint8: cannot restore to {}", dtype)
+        _need(self.whole(), "checkpoint8: codes {} and exponents {} do not hold an activation {}", tuple(self.codes.shape), tuple(self.exps.shape), self.shape)
+        _one_device(self.codes, self.exps)
         out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
         if out.numel():
             _launch(_library().sn_checkpoint8_restore, "sn_checkpoint8_restore", out.device, _p(self.codes), _p(self.exps), self.codes.shape[0],
@@ -133,10 +143,7 @@ class Checkpoint8:
 
 def _empty_checkpoint(shape, dtype, dev):
     n = shape[-1]
-    rows = 1
-    for s in shape[:-1]:
-        rows *= s
-    npad = (n + 31) // 32 * 32
+    rows, npad = math.prod(shape[:-1]), (n + 31) // 32 * 32
     return Checkpoint8(torch.empty((rows, npad), dtype=torch.int8, device=dev), torch.empty((rows, npad // 32), dtype=torch.uint8, device=dev), shape, dtype)
 
 
@@ -160,7 +167,8 @@ def checkpoint8_weight_grad(dy, kept, bias=True, out_dtype=None):
     kept = checkpoint8(x) of x [..., in] with the same leading sizes -> (dW [out, in], db [out] or None).
 
     dW = sum_r dy[r]^T kept[r] on the bf16 matrix cores with float32 sums.  The kept values are exact in bf16 and dy enters as
-    bf16 pieces that add up to it (float32: three, float16: two), so the products carry no rounding of their own.
+    bf16 pieces that add up to it (float32: three, float16: two), so the products carry no rounding of their own.  A gradient that is
+    infinite or NaN (float32: or beyond bfloat16's largest, 3.39e38) makes its feature's row of dW infinite or NaN.
     out_dtype: the type of both results (default dy's)."""
     _need(isinstance(kept, Checkpoint8), "checkpoint8_weight_grad: expected a Checkpoint8, got {}", type(kept).__name__)
     _need(torch.is_tensor(dy) and dy.dtype in _TYPES, "checkpoint8_weight_grad: expected float32, bfloat16 or float16 gradients")
@@ -168,7 +176,9 @@ def checkpoint8_weight_grad(dy, kept, bias=True, out_dtype=None):
     _need(out_dtype in _TYPES, "checkpoint8_weight_grad: cannot write {}", out_dtype)
     _need(dy.dim() >= 2 and dy.shape[-1] >= 1 and tuple(dy.shape[:-1]) == kept.shape[:-1],
           "checkpoint8_weight_grad: gradients {} do not fit the activation {}", tuple(dy.shape), kept.shape)
-    dev = _one_device(dy, kept.codes)
+    _need(kept.whole(), "checkpoint8_weight_grad: codes {} and exponents {} do not hold an activation {}", tuple(kept.codes.shape), tuple(kept.exps.shape),
+          kept.shape)
+    dev = _one_device(dy, kept.codes, kept.exps)
     dy = dy.detach()
     out_f, in_f, rows = dy.shape[-1], kept.shape[-1], kept.codes.shape[0]
     if rows == 0:
@@ -381,7 +391,7 @@ def gated_residual_norms(x, branch, gate=None, scale=None, post=None, pre=None, 
                 params[i] = t.contiguous()
     if eps < 0:
         _need(False, "gated_residual_norms: eps {}", eps)
-    if n_valid is not None and not (x.dim() == 3 and n_valid.dtype == torch.int32 and n_valid.shape == shape[:1] and n_valid.is_contiguous()):
+    if n_valid is not None and not (torch.is_tensor(n_valid) and x.dim() == 3 and n_valid.dtype == torch.int32 and n_valid.shape == shape[:1] and n_valid.is_contiguous()):
         _need(False, "gated_residual_norms: n_valid must be int32 [G] with x [G, n, width]")
     _one_device(x, branch, gate, n_valid, *params)
     if types == torch.float64:
@@ -453,7 +463,8 @@ def label_log_probs(logits, target, topk=0, ignore_index=-100):
         entropy [...] float32: -sum p log p (entries at -inf count as 0)
         top_log_probs, top_ids [..., topk]: the topk largest, the lowest index first among equals (None for topk = 0; at most 64)
     log_probs and entropy are differentiable in the logits, the alternatives are not.  A row of -inf only has no distribution: log_probs
-    and top_log_probs -inf, entropy 0, no gradient.  A NaN or +inf logit makes its row's results NaN."""
+    and top_log_probs -inf, entropy 0, no gradient.  A NaN or +inf logit makes its row's results NaN; a row whose upstream gradients are
+    zeros (an ignored target) gets zeros, whatever its logits.  Under 2^24 rows of under 2^30 entries."""
     if not torch.is_tensor(logits) or logits.dtype not in _TYPES or logits.dim() < 1:
         _need(False, "label_log_probs: expected float32, bfloat16 or float16 logits")
     if not torch.is_tensor(target) or target.dtype != torch.int64 or target.shape != logits.shape[:-1]:

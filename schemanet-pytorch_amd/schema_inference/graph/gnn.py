@@ -420,11 +420,11 @@ class GNN(nn.Module):
         first = self.layers[0].norm if len(self.layers) else self.out_norm
         if E <= 1024 and x.is_cuda:
             h = ops.mask_layernorm_act(x, first.weight, first.bias, first.eps, n_valid=n_valid, relu=False)
-            if n_valid is not None:
-                # (that op norms a padding row as a row of zeros: its bias; here padding is zero throughout)
-                h = h.masked_fill((torch.arange(n, device=h.device)[None, :] >= n_valid[:, None])[..., None], 0.0)
         else:
             h = first(x)
+        if n_valid is not None:
+            # (these norms leave their bias in a padding row; here padding is zero throughout)
+            h = h.masked_fill((torch.arange(n, device=h.device)[None, :] >= n_valid[:, None])[..., None], 0.0)
         for i, layer in enumerate(self.layers):
             summed = ops.edges_adj_matmul(edges, h, planes, True) if planes is not None else torch.bmm(adj, h)
             branch = layer.activation(self._residual_linear(layer.g_conv.linear, summed))

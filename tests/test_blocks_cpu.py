@@ -139,6 +139,41 @@ def test_checkpoint8_refuses(ops):
         ops.checkpoint8_weight_grad(torch.zeros(2, 3, 5), kept)
 
 
+@pytest.mark.parametrize("codes,exps", [
+    (torch.zeros(5, 32, dtype=torch.int8), torch.zeros(6, 1, dtype=torch.uint8)),             # fewer rows
+    (torch.zeros(7, 32, dtype=torch.int8), torch.zeros(7, 1, dtype=torch.uint8)),             # more
+    (torch.zeros(6, 20, dtype=torch.int8), torch.zeros(6, 1, dtype=torch.uint8)),             # not padded
+    (torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 0, dtype=torch.uint8)),
+    (torch.zeros(6, 32, dtype=torch.int8), torch.zeros(3, 1, dtype=torch.uint8)),
+    (torch.zeros(6, 64, dtype=torch.int8)[:, ::2], torch.zeros(6, 1, dtype=torch.uint8)),
+    (torch.zeros(6, 32, dtype=torch.uint8), torch.zeros(6, 1, dtype=torch.uint8)),
+    (torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 1)),
+])
+def test_checkpoint8_of_another_layout_is_refused(ops, codes, exps):
+    kept = ops.Checkpoint8(codes, exps, (2, 3, 20), torch.float32)
+    with pytest.raises(RuntimeError, match="do not hold"):
+        kept.restore()
+    with pytest.raises(RuntimeError, match="do not hold"):
+        ops.checkpoint8_weight_grad(torch.zeros(2, 3, 5), kept)
+
+
+def test_ce_entropy_loss_ignores_rows():
+    """ignored rows count for nothing, whatever stands in them"""
+    from schema_inference.loss import CEEntropyLoss
+    x = torch.randn(6, 9, generator=torch.Generator().manual_seed(2))
+    x[0, 3:5] = float("-inf")
+    x[1], x[2, 0], x[4] = float("nan"), float("-inf"), float("-inf")
+    label = torch.tensor([1, -100, -100, 4, -100, 8])
+    used = label != -100
+    leaf, alone = x.clone().requires_grad_(), x[used].clone().requires_grad_()
+    got, want = CEEntropyLoss()({"pred": leaf}, {"label": label}), CEEntropyLoss()({"pred": alone}, {"label": label[used]})
+    tol = 8 * 2.0 ** -24                                            # sums of three terms of size under 8, in another order
+    assert all(abs(float((got[k] - want[k]).detach())) <= 8 * tol for k in ("cls", "entropy"))
+    g1, = torch.autograd.grad(got["cls"] + got["entropy"], leaf)
+    g2, = torch.autograd.grad(want["cls"] + want["entropy"], alone)
+    assert not bool(g1[~used].any()) and float((g1[used] - g2).abs().max()) <= tol
+
+
 def test_linear_checkpoint8_refuses(ops):
     x, w = torch.zeros(4, 32), torch.zeros(16, 32)
     with pytest.raises(RuntimeError, match="weight"):
@@ -177,6 +212,11 @@ def test_gated_residual_norms_refuses(ops):
         call(x[0], x[0], n_valid=torch.zeros(3, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         call(x, x, post=(v, v))
+
+
+def test_extents_that_are_not_a_tensor_are_refused(ops):
+    with pytest.raises(RuntimeError, match="n_valid"):
+        ops.gated_residual_norms(torch.zeros(2, 3, 8), torch.zeros(2, 3, 8), n_valid=[1, 2])
 
 
 def test_label_log_probs_refuses(ops):
