@@ -112,28 +112,45 @@ class Checkpoint8:
     as round(x / s) (half to even): off by at most s / 2 <= max|x| / 127.5, up to max|x| / 254 where the maximum is just under
     127.5 s.  A block that held an infinity or a NaN comes back as NaN; magnitudes under 2^-126 as zero."""
 
-    __slots__ = ("codes", "exps", "shape", "dtype")
+    __slots__ = ("_codes", "_exps", "_shape", "dtype")
 
     def __init__(self, codes, exps, shape, dtype):
-        self.codes, self.exps, self.shape, self.dtype = codes, exps, tuple(shape), dtype
+        # (checked here, once: the kernels read both by the shape, and none of the three can be replaced later)
+        shape = tuple(shape)
+        _need(len(shape) >= 1 and shape[-1] >= 1, "checkpoint8: expected at least one feature, got shape {}", shape)
+        rows, npad = math.prod(shape[:-1]), (shape[-1] + 31) // 32 * 32
+        _need(codes.dtype == torch.int8 and exps.dtype == torch.uint8 and codes.shape == (rows, npad) and exps.shape == (rows, npad // 32)
+              and codes.is_contiguous() and exps.is_contiguous() and codes.device == exps.device,
+              "checkpoint8: codes {} and exponents {} do not hold an activation {}", tuple(codes.shape), tuple(exps.shape), shape)
+        self._codes, self._exps, self._shape, self.dtype = codes, exps, shape, dtype
+
+    @classmethod
+    def _of(cls, codes, exps, shape, dtype):
+        """without the checks: buffers that this module has made"""
+        self = cls.__new__(cls)
+        self._codes, self._exps, self._shape, self.dtype = codes, exps, tuple(shape), dtype
+        return self
+
+    @property
+    def codes(self):
+        return self._codes
+
+    @property
+    def exps(self):
+        return self._exps
+
+    @property
+    def shape(self):
+        return self._shape
 
     @property
     def nbytes(self):
         return self.codes.numel() + self.exps.numel()
 
-    def whole(self):
-        """do codes and exponents have the layout that `shape` asks for?  (the kernels read them by it)"""
-        n, codes, exps = self.shape[-1], self.codes, self.exps
-        rows, npad = math.prod(self.shape[:-1]), (n + 31) // 32 * 32
-        return (codes.dtype == torch.int8 and exps.dtype == torch.uint8 and codes.shape == (rows, npad) and exps.shape == (rows, npad // 32)
-                and codes.is_contiguous() and exps.is_contiguous())
-
     def restore(self, dtype=None):
         """the kept values, [..., n] in `dtype` (default: the type of the activation; bfloat16 and float32 hold them exactly)"""
         dtype = dtype or self.dtype
         _need(dtype in _TYPES, "checkpoint8: cannot restore to {}", dtype)
-        _need(self.whole(), "checkpoint8: codes {} and exponents {} do not hold an activation {}", tuple(self.codes.shape), tuple(self.exps.shape), self.shape)
-        _one_device(self.codes, self.exps)
         out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
         if out.numel():
             _launch(_library().sn_checkpoint8_restore, "sn_checkpoint8_restore", out.device, _p(self.codes), _p(self.exps), self.codes.shape[0],
@@ -144,7 +161,7 @@ class Checkpoint8:
 def _empty_checkpoint(shape, dtype, dev):
     n = shape[-1]
     rows, npad = math.prod(shape[:-1]), (n + 31) // 32 * 32
-    return Checkpoint8(torch.empty((rows, npad), dtype=torch.int8, device=dev), torch.empty((rows, npad // 32), dtype=torch.uint8, device=dev), shape, dtype)
+    return Checkpoint8._of(torch.empty((rows, npad), dtype=torch.int8, device=dev), torch.empty((rows, npad // 32), dtype=torch.uint8, device=dev), shape, dtype)
 
 
 def checkpoint8(x):
@@ -176,9 +193,7 @@ def checkpoint8_weight_grad(dy, kept, bias=True, out_dtype=None):
     _need(out_dtype in _TYPES, "checkpoint8_weight_grad: cannot write {}", out_dtype)
     _need(dy.dim() >= 2 and dy.shape[-1] >= 1 and tuple(dy.shape[:-1]) == kept.shape[:-1],
           "checkpoint8_weight_grad: gradients {} do not fit the activation {}", tuple(dy.shape), kept.shape)
-    _need(kept.whole(), "checkpoint8_weight_grad: codes {} and exponents {} do not hold an activation {}", tuple(kept.codes.shape), tuple(kept.exps.shape),
-          kept.shape)
-    dev = _one_device(dy, kept.codes, kept.exps)
+    dev = _one_device(dy, kept.codes)
     dy = dy.detach()
     out_f, in_f, rows = dy.shape[-1], kept.shape[-1], kept.codes.shape[0]
     if rows == 0:
@@ -223,7 +238,7 @@ class _LinearCheckpoint8(torch.autograd.Function):
             dx = ops.gcn_gemm(ops.split_planes(dy3), ops.split_planes(weight.detach(), scale=ctx.scale, transpose=True), dy3.shape[0], want_c=True)["c"]
             dx = dx[0] if len(ctx.shape) == 2 else dx
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            kept = Checkpoint8(ctx.saved_tensors[1], ctx.saved_tensors[2], ctx.shape, torch.float32)
+            kept = Checkpoint8._of(ctx.saved_tensors[1], ctx.saved_tensors[2], ctx.shape, torch.float32)
             dw, db = checkpoint8_weight_grad(dy3[0] if len(ctx.shape) == 2 else dy3, kept, bias=ctx.has_bias)
             dw = dw if ctx.needs_input_grad[1] else None
         return dx, dw, db

@@ -150,11 +150,17 @@ def test_checkpoint8_refuses(ops):
     (torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 1)),
 ])
 def test_checkpoint8_of_another_layout_is_refused(ops, codes, exps):
-    kept = ops.Checkpoint8(codes, exps, (2, 3, 20), torch.float32)
     with pytest.raises(RuntimeError, match="do not hold"):
-        kept.restore()
-    with pytest.raises(RuntimeError, match="do not hold"):
-        ops.checkpoint8_weight_grad(torch.zeros(2, 3, 5), kept)
+        ops.Checkpoint8(codes, exps, (2, 3, 20), torch.float32)
+
+
+def test_a_checkpoint8_stays_whole(ops):
+    kept = ops.Checkpoint8(torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 1, dtype=torch.uint8), (2, 3, 20), torch.float32)
+    for name in ("codes", "exps", "shape"):
+        with pytest.raises(AttributeError):
+            setattr(kept, name, getattr(kept, name)[:1])
+    with pytest.raises(RuntimeError, match="at least one feature"):
+        ops.Checkpoint8(kept.codes, kept.exps, (6, 0), torch.float32)
 
 
 def test_ce_entropy_loss_ignores_rows():
