@@ -8,6 +8,8 @@ reference cpp_extension/__init__.py:5-10); here the binding is ctypes over plain
 torch used only to own device memory and provide the current HIP stream.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import subprocess
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
@@ -22,7 +24,9 @@ ABI_VERSION = 12
 # signature or a struct without a new hash here - and, by the rule in the header, a new ABI_VERSION - fails the CPU suite.
 ABI_HEADER_SHA = "cfb9f51fec2f16d9"
 SN_MAX_TOKENS = 196
+BLOCKS_PATH = os.path.join(_PKG, "lib", "_schemanet_blocks.so")
 _lib = None
+_blocks = None
 
 
 class _SizedArgs(Structure):
@@ -226,8 +230,8 @@ BLOCK_SYMBOLS = tuple(_BLOCK_SIGNATURES)
 
 def build(force=False):
     """hipcc-compile the library in-tree (cross-compiles for gfx950 without a GPU)."""
-    if force or not os.path.exists(LIB_PATH):
-        subprocess.check_call(["make", "-s", "-C", _PKG, "lib/libschemanet_hip.so"])
+    if force or not (os.path.exists(LIB_PATH) and os.path.exists(BLOCKS_PATH)):
+        subprocess.check_call(["make", "-s", "-C", _PKG, "all"])
     return LIB_PATH
 
 
@@ -260,6 +264,28 @@ def require_gpu():
                            "there is no CPU fallback")
     lib = load()
     return lib
+
+
+# entry points in the order in which csrc/sn_torch.cpp binds them
+_BOUND = ("sn_last_error", "sn_checkpoint8", "sn_checkpoint8_restore", "sn_checkpoint8_weight_grad_workspace", "sn_checkpoint8_weight_grad",
+          "sn_block_norms_forward", "sn_block_norms_workspace", "sn_block_norms_backward", "sn_label_log_probs_workspace", "sn_label_log_probs",
+          "sn_label_log_probs_backward")
+
+
+def blocks():
+    """The module of csrc/sn_torch.cpp (torch's side of include/schemanet_blocks.h), bound to the loaded library."""
+    global _blocks
+    if _blocks is None:
+        lib = load()
+        if not os.path.exists(BLOCKS_PATH):
+            raise RuntimeError(f"schemanet HIP extension not built: {BLOCKS_PATH} is missing (run `python -c 'import __graft_entry__ as g; "
+                               f"g.build()'` or `make -C schemanet-pytorch_amd`); there is no CPU fallback")
+        loader = importlib.machinery.ExtensionFileLoader("_schemanet_blocks", BLOCKS_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_schemanet_blocks", loader))
+        loader.exec_module(module)
+        module.bind(tuple(ctypes.cast(getattr(lib, name), c_void_p).value for name in _BOUND), require_gpu)
+        _blocks = module
+    return _blocks
 
 
 def check(rc, what=""):
