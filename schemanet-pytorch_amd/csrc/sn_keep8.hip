@@ -39,10 +39,12 @@ __global__ __launch_bounds__(kPackThreads) void checkpoint8_kernel(const void *x
     }
 }
 
+// HBM bound: 16 bytes of the result a lane (fp32 32 bytes, 16-bit types 8: slower both at 12544 rows of 256, 4.9 -> 5.4 us and 3.5 -> 4.3, and at
+// 32768 rows of 2048, 69 -> 94 and 31.8 -> 34.3; the latter, bf16, is 6.3 TB/s)
 template <int DT>
 __global__ __launch_bounds__(kPackThreads) void restore8_kernel(const uint8_t *codes, const uint8_t *exps, int64_t rows, int n, void *out)
 {
-    constexpr int EV = DT == SN_F32 ? 4 : 8;                 // 16 bytes of the result a lane
+    constexpr int EV = DT == SN_F32 ? 4 : 8;
     const int npad = (n + 31) & ~31, groups = (n + EV - 1) / EV;
     const int64_t total = rows * groups, turn = (int64_t)gridDim.x * kPackThreads;
     for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < total; i += turn) {

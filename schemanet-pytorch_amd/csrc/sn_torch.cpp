@@ -115,14 +115,22 @@ Rows rows_of(const Tensor &t, int64_t width)
     return {t, stride < 0 ? width : stride};
 }
 
-// results of a backward pass that was asked for its own graph: using them for second derivatives raises
-variable_list without_second(variable_list grads)
+// Results of a backward pass that was asked for its own graph: whoever differentiates them, with respect to the node's inputs or to the
+// upstream gradients, gets an error.
+variable_list without_second(const torch::autograd::Node &node, const variable_list &upstream, variable_list out)
 {
-    if (!at::GradMode::is_enabled()) return grads;
-    variable_list marked;
-    for (const Tensor &g : grads) marked.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
-    torch::autograd::DelayedError error("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)marked.size());
-    return error(std::move(marked));
+    if (!at::GradMode::is_enabled()) return out;
+    torch::autograd::edge_list edges = node.next_edges();
+    for (const Tensor &g : upstream)
+        if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+    const std::shared_ptr<torch::autograd::Node> error(new torch::autograd::Error(node.name() + ": no second derivatives", std::move(edges)),
+                                                       torch::autograd::deleteNode);
+    for (Tensor &t : out) {
+        if (!t.defined()) continue;
+        t = t.detach();
+        torch::autograd::set_history(t, error);
+    }
+    return out;
 }
 
 // -------------------------------------------------------------------------------------------------------------------- norms
@@ -180,7 +188,7 @@ struct GatedResidualNormsBackward : torch::autograd::Node {
             at::AutoDispatchBelowADInplaceOrView raw;
             run(grads[0], grads.size() > 1 ? grads[1] : Tensor(), out);
         }
-        return without_second(std::move(out));
+        return without_second(*this, grads, std::move(out));
     }
 
     void run(const Tensor &dy, const Tensor &dh, variable_list &out)
@@ -359,7 +367,7 @@ struct LabelLogProbsBackward : torch::autograd::Node {
                       "sn_label_log_probs_backward");
             }
         }
-        return without_second(std::move(out));
+        return without_second(*this, grads, std::move(out));
     }
 };
 

@@ -735,6 +735,90 @@ def test_only_what_is_asked_for(ops):
     y.sum().backward()
 
 
+def both(ops, t, keep8=False):
+    """-> leaves and the results of both differentiable operators"""
+    leaves = [v.clone().requires_grad_() for v in (t["x"], t["branch"], t["gate"], t["scale"], *t["post"], *t["pre"])]
+    x, branch, gate, scale, pw, pb, w, b = leaves
+    y, h = ops.gated_residual_norms(x, branch, gate=gate, scale=scale, post=(pw, pb), pre=(w, b), checkpoint8=keep8)
+    got = ops.label_log_probs(h, torch.arange(h.shape[0], device=DEV) % h.shape[1])
+    return leaves, [y, got.log_probs, got.entropy]
+
+
+def grads_of(leaves, out, **how):
+    return torch.autograd.grad(out, leaves, [torch.ones_like(o) * (i + 1) for i, o in enumerate(out)], **how)
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+def test_backward_twice_and_through_hooks(ops, keep8):
+    """a kept graph gives the same gradients again, a freed one raises; what is saved goes through the hooks for saved tensors"""
+    t = norm_inputs(gen(31), (40, 200), F32)
+    leaves, out = both(ops, t, keep8)
+    first = grads_of(leaves, out, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, grads_of(leaves, out)))
+    with pytest.raises(RuntimeError, match="second time"):
+        grads_of(leaves, out)
+    with torch.autograd.graph.save_on_cpu():
+        leaves, out = both(ops, t, keep8)
+    assert all(torch.equal(a, b) for a, b in zip(first, grads_of(leaves, out)))
+    leaves, out = both(ops, t, keep8)
+    for o, leaf in ((out, leaves),):
+        torch.autograd.backward(o, [torch.ones_like(v) * (i + 1) for i, v in enumerate(o)])
+        assert all(torch.equal(a, v.grad) for a, v in zip(first, leaf))
+    seen = []
+    leaves, out = both(ops, t, keep8)
+    leaves[0].register_hook(lambda g: seen.append(g.clone()))
+    grads_of(leaves, out)
+    assert torch.equal(seen[0], first[0])
+
+
+def test_inputs_changed_before_the_backward_pass(ops):
+    """an input that the backward pass refers to must not change in between; with checkpoints it may"""
+    t = norm_inputs(gen(32), (20, 64), F32)
+    for keep8 in (False, True):
+        x = t["x"].clone()
+        branch = t["branch"].clone().requires_grad_()
+        y, h = ops.gated_residual_norms(x, branch, post=t["post"], pre=t["pre"], checkpoint8=keep8)
+        before, = torch.autograd.grad(h.sum() + (y * y).sum(), branch, retain_graph=True)
+        again = h.sum() + (y * y).sum()
+        x.zero_()
+        if keep8:
+            assert torch.equal(before, torch.autograd.grad(again, branch)[0])
+        else:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(again, branch)
+
+
+def test_without_gradients(ops):
+    t = norm_inputs(gen(33), (20, 64), F32)
+    x = t["x"].clone().requires_grad_()
+    want = ops.gated_residual_norms(x, t["branch"], post=t["post"], pre=t["pre"])
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            y, h = ops.gated_residual_norms(x, t["branch"], post=t["post"], pre=t["pre"])
+            got = ops.label_log_probs(h, torch.zeros(20, dtype=torch.int64, device=DEV), topk=2)
+        assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+        assert not any(v.requires_grad for v in (y, h, *got))
+    plain = ops.gated_residual_norms(t["x"], t["branch"], post=t["post"])
+    assert plain[1] is None and not plain[0].requires_grad
+
+
+def test_second_derivatives_are_refused(ops):
+    t = norm_inputs(gen(34), (20, 64), F32)
+    leaves, out = both(ops, t)
+    first = grads_of(leaves, out)
+    leaves, out = both(ops, t)
+    graph = grads_of(leaves, out, create_graph=True)
+    assert all(torch.equal(a, b.detach()) for a, b in zip(first, graph))
+    for g in graph:
+        with pytest.raises(RuntimeError, match="no second derivatives"):
+            torch.autograd.grad(g.sum(), leaves, allow_unused=True, retain_graph=True)
+    leaves, out = both(ops, t)
+    up = [torch.ones_like(o).requires_grad_() for o in out]
+    g, = torch.autograd.grad(out, leaves[:1], up, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivatives"):
+        torch.autograd.grad(g.sum(), up)
+
+
 def test_long_rows_pass_32_bit_offsets(ops):
     """an activation of more than 2^32 bytes: the last rows are where they should be"""
     rows, n = (1 << 21) + 3, 1056
