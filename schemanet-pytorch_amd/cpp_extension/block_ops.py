@@ -152,6 +152,7 @@ def linear_checkpoint8(x, weight, bias=None):
     for t in (x, weight, bias):
         _need(t is None or t.is_cuda, "expected CUDA tensors (the HIP path has no CPU fallback)")
         _need(t is None or t.device == x.device, "tensors on different devices: {} vs {}", x.device, None if t is None else t.device)
+    N.blocks().before_capture(x, weight, bias)
     return _LinearCheckpoint8.apply(x, weight, bias)
 
 

@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/function.h>
@@ -113,6 +114,19 @@ Rows rows_of(const Tensor &t, int64_t width)
         next = t.stride(d) * t.size(d);
     }
     return {t, stride < 0 ? width : stride};
+}
+
+// A backward pass captured into a graph must not reach autograd nodes of the default stream, which cannot take part in a capture: those
+// that an eager graph of the same leaves keeps alive.  The engine would find out on its own thread and end the process.
+void before_capture(const torch::autograd::edge_list &edges, const char *who)
+{
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const torch::autograd::Edge &e : edges) {
+        if (!e.is_valid()) continue;
+        const auto stream = e.function->stream();
+        if (stream && stream->id() == 0)
+            refuse("%s: captured into a graph while an autograd graph of the default stream uses the same tensors (drop its results first)", who);
+    }
 }
 
 // Results of a backward pass that was asked for its own graph: whoever differentiates them, with respect to the node's inputs or to the
@@ -316,6 +330,7 @@ std::pair<Tensor, Tensor> gated_residual_norms(const Tensor &x, const Tensor &br
     if (train) {
         node = std::shared_ptr<GatedResidualNormsBackward>(new GatedResidualNormsBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x, branch, gate, p[0], p[1], p[2], p[3], p[4]));
+        before_capture(node->next_edges(), "gated_residual_norms");
     }
     NormsResult r = norms_forward(c, x, branch, gate, train, keep8);
     if (train) {
@@ -387,6 +402,7 @@ Scores label_log_probs(const Tensor &logits, const Tensor &given, int64_t topk, 
     if (at::GradMode::is_enabled() && logits.requires_grad()) {
         node = std::shared_ptr<LabelLogProbsBackward>(new LabelLogProbsBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(logits));
+        before_capture(node->next_edges(), "label_log_probs");
     }
     Scores o;
     Tensor target, stats;
@@ -608,6 +624,15 @@ PyObject *py_weight_grad(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
+// before_capture(x, weight, bias) of linear_checkpoint8, whose node is Python's
+PyObject *py_before_capture(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return guarded(n, 3, [&]() -> PyObject * {
+        if (at::GradMode::is_enabled()) before_capture(torch::autograd::collect_next_edges(tensor(a[0]), tensor(a[1]), tensor(a[2])), "linear_checkpoint8");
+        Py_RETURN_NONE;
+    });
+}
+
 // bind(addresses of the entry points in Library's order, what to call before the first launch)
 PyObject *py_bind(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
@@ -629,6 +654,7 @@ PyMethodDef methods[] = {SN_METHOD("bind", py_bind),
                          SN_METHOD("checkpoint8", py_checkpoint8),
                          SN_METHOD("restore", py_restore),
                          SN_METHOD("weight_grad", py_weight_grad),
+                         SN_METHOD("before_capture", py_before_capture),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_schemanet_blocks", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

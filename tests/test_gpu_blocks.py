@@ -802,6 +802,39 @@ def test_without_gradients(ops):
     assert plain[1] is None and not plain[0].requires_grad
 
 
+def test_capture_beside_an_eager_graph_is_refused(ops):
+    """the forward call says so: the backward pass could not be captured.  (It is not called here.)  With the eager graph gone it can"""
+    t = norm_inputs(gen(35), (20, 64), F32)
+    w = rand(gen(36), 64, 64).requires_grad_()
+    x, logits = t["x"].clone().requires_grad_(), rand(gen(37), 20, 50).requires_grad_()
+    target = torch.arange(20, device=DEV)
+    calls = {"gated_residual_norms": lambda: ops.gated_residual_norms(x, t["branch"], post=t["post"])[0],
+             "label_log_probs": lambda: ops.label_log_probs(logits, target).log_probs,
+             "linear_checkpoint8": lambda: ops.linear_checkpoint8(t["branch"], w)}
+    for name, call in calls.items():
+        leaf = {"gated_residual_norms": x, "label_log_probs": logits, "linear_checkpoint8": w}[name]
+        alive = call()
+        want = torch.autograd.grad(alive.sum(), leaf, retain_graph=True)[0]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match=name + ".*captured"):
+                call()
+        del alive, graph
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(call().sum(), leaf)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(call().sum(), leaf)[0]
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
 def test_second_derivatives_are_refused(ops):
     t = norm_inputs(gen(34), (20, 64), F32)
     leaves, out = both(ops, t)
