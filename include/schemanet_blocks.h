@@ -98,7 +98,8 @@ int sn_label_log_probs(const void *logits, int dtype, int64_t rows, int64_t n, i
                        int k, float *log_probs, float *entropy, float *stats, float *top_log_probs, int64_t *top_ids, void *workspace,
                        size_t workspace_bytes, void *stream);
 /* grad [rows, n] contiguous, in the logits' type: g_log_probs[r] (delta(target) - p) - g_entropy[r] p (log p + entropy);
- * either upstream gradient may be NULL. */
+ * either upstream gradient may be NULL.  A row whose upstream gradients are zeros (g_log_probs of an ignored target counts as zero) is
+ * not read and gets zeros, unless its target lies outside. */
 int sn_label_log_probs_backward(const void *logits, int dtype, int64_t rows, int64_t n, int64_t row_stride, const int64_t *target,
                                 int64_t ignore_index, const float *stats, const float *g_log_probs, const float *g_entropy, void *grad,
                                 void *stream);

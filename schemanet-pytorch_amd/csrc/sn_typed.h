@@ -12,10 +12,6 @@ namespace sn {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-template <int DT> struct Elem { typedef float type; };
-template <> struct Elem<SN_BF16> { typedef uint16_t type; };
-template <> struct Elem<SN_F16> { typedef _Float16 type; };
-
 __device__ __forceinline__ float bf16_to_f32(uint32_t u) { return __uint_as_float(u << 16); }
 // two floats -> two bf16 in one word, round to nearest even (v_cvt_pk_bf16_f32)
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b)
@@ -116,11 +112,7 @@ template <int DT> __device__ __forceinline__ void store_one(void *p, int64_t i, 
     else if constexpr (DT == SN_BF16) ((uint16_t *)p)[i] = (uint16_t)(pack_bf16(v, 0.0f) & 0xFFFFu);
     else ((_Float16 *)p)[i] = (_Float16)v;
 }
-// the type as a (uniform) run-time value: parameters and their gradients
-__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i)
-{
-    return dtype == SN_F32 ? load_one<SN_F32>(p, i) : dtype == SN_BF16 ? load_one<SN_BF16>(p, i) : load_one<SN_F16>(p, i);
-}
+// the type as a (uniform) run-time value: gradients of parameters
 __device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v)
 {
     if (dtype == SN_F32) store_one<SN_F32>(p, i, v);
