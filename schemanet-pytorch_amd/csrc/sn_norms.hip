@@ -240,10 +240,12 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
     return s;
 }
 
-// MODE: 0 = the parts of the call are looked up at run time; 1 = everything is there (2: but the gate).  The branches of mode 0 make the
-// compiler wait for all loads and stores in flight where it needs the oldest row, the straight line of the others does not
-// (backward of 32768 rows of 4096 bf16: 761 us looked up and one row ahead, 427 straight and two ahead).  For the same reason rows that
-// do not count are passed over by scalar arithmetic, and get their zeros in a loop of their own.
+// MODE: 0 = the parts of the call are looked up at run time; otherwise the sum of those that are there: 1 the gate, 2 the norm after the
+// block, 4 the norm before the next one.  The branches of mode 0 make the compiler wait for all loads and stores in flight where it needs
+// the oldest row, the straight lines of the others do not (us, forward / backward, looked up and straight: bf16, 131072 rows of 1024, all
+// parts 268 / 464 and 263 / 408, both norms 253 / 410 and 216 / 312, the second alone 215 / 357 and 191 / 309, the first alone 180 / 327 and 141 / 242 (x is not read); 32768 rows of 4096, all
+// parts 326 / 464 and 306 / 418; fp32, 103424 rows of 256 118 / 162 and 108 / 161).  For the same reason rows that do not count are passed
+// over by scalar arithmetic, and get their zeros in a loop of their own.
 template <int DT, int EV, int CH, bool MULTI, int MODE, bool KEEP>
 __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block_norms_args a)
 {
@@ -259,7 +261,7 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block
     const int t = MULTI ? threadIdx.x : threadIdx.x & 63;
     const int E = a.width, step = (MULTI ? (int)blockDim.x : 64) * EV, col = t * EV, npad = (E + 31) & ~31;
     const float inv_e = 1.0f / (float)E;
-    const bool gated = ALL ? MODE == 1 : a.gate != nullptr, post = ALL || a.has_post, pre = ALL || a.has_pre;
+    const bool gated = ALL ? MODE & 1 : a.gate != nullptr, post = ALL ? MODE & 2 : a.has_post != 0, pre = ALL ? MODE & 4 : a.has_pre != 0;
     const bool tail = __any(tail_shift<EV>(col + (CH - 1) * step, E) > 0);
     const int64_t turn = (int64_t)gridDim.x * L::kRows;
 
@@ -358,8 +360,8 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
     const int t = MULTI ? threadIdx.x : threadIdx.x & 63;
     const int E = a.width, step = (MULTI ? (int)blockDim.x : 64) * EV, col = t * EV, npad = (E + 31) & ~31;
     const float inv_e = 1.0f / (float)E;
-    const bool gated = ALL ? MODE == 1 : KEPT ? a.gate_codes != nullptr : a.gate != nullptr;
-    const bool post = ALL || a.has_post, has_dy = ALL || a.dy, has_dh = ALL || a.dh;
+    const bool gated = ALL ? MODE & 1 : KEPT ? a.gate_codes != nullptr : a.gate != nullptr;
+    const bool post = ALL ? MODE & 2 : a.has_post != 0, has_dy = ALL || a.dy, has_dh = ALL ? MODE & 4 : a.dh != nullptr;
     const bool tail = __any(tail_shift<EV>(col + (CH - 1) * step, E) > 0);
     const int64_t turn = (int64_t)gridDim.x * L::kRows;
 
@@ -583,6 +585,12 @@ int check_args(const sn_block_norms_args *a, const char *who)
     return SN_OK;
 }
 
+// rest: whatever else a straight-line kernel takes for granted (without any norm there is none: index 1 of the tables is mode 0 too)
+int mode_of(const sn_block_norms_args &a, const void *gate, bool rest) { return rest ? (gate ? 1 : 0) + (a.has_post ? 2 : 0) + (a.has_pre ? 4 : 0) : 0; }
+#define SN_NORMS_MODES(kernel, kept) \
+    {kernel<DT, EV, CH, MULTI, 0, kept>, kernel<DT, EV, CH, MULTI, 0, kept>, kernel<DT, EV, CH, MULTI, 2, kept>, kernel<DT, EV, CH, MULTI, 3, kept>, \
+     kernel<DT, EV, CH, MULTI, 4, kept>, kernel<DT, EV, CH, MULTI, 5, kept>, kernel<DT, EV, CH, MULTI, 6, kept>, kernel<DT, EV, CH, MULTI, 7, kept>}
+
 template <int DT, int EV, int CH, bool MULTI> int launch_forward(const sn_block_norms_args &a, hipStream_t st)
 {
     using L = Layout<DT, EV, CH, MULTI>;
@@ -591,11 +599,9 @@ template <int DT, int EV, int CH, bool MULTI> int launch_forward(const sn_block_
     // fp32 103424 x 256 with 4, 8, 16, 32: 100 109 108 116, bf16 200000 x 256 with 2, 4, 8, 16: 134 106 109 103).
     const int W = waves_for(a.width);
     const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = 256 * (MULTI ? (8 + W - 1) / W : 8), each = (turns + most - 1) / most;
-    const bool all = a.has_post && a.has_pre;
-    const auto kernel = a.x_codes ? (!all ? norms_forward_kernel<DT, EV, CH, MULTI, 0, true> : a.gate ? norms_forward_kernel<DT, EV, CH, MULTI, 1, true>
-                                                                                                      : norms_forward_kernel<DT, EV, CH, MULTI, 2, true>)
-                                  : (!all ? norms_forward_kernel<DT, EV, CH, MULTI, 0, false> : a.gate ? norms_forward_kernel<DT, EV, CH, MULTI, 1, false>
-                                                                                                       : norms_forward_kernel<DT, EV, CH, MULTI, 2, false>);
+    using Kernel = void (*)(sn_block_norms_args);
+    static constexpr Kernel kernels[2][8] = {SN_NORMS_MODES(norms_forward_kernel, false), SN_NORMS_MODES(norms_forward_kernel, true)};
+    const Kernel kernel = kernels[a.x_codes != nullptr][mode_of(a, a.gate, true)];
     hipLaunchKernelGGL(kernel, dim3((unsigned)((turns + each - 1) / each)), dim3(MULTI ? waves_for(a.width) * 64 : 256), 0, st, a);
     SN_CHECK_LAUNCH("sn_block_norms_forward");
     return SN_OK;
@@ -607,12 +613,11 @@ template <int DT, int EV, int CH, bool MULTI> int launch_backward(const sn_block
     bool columns = false;
     for (int k = 0; k < kVectors; ++k) columns |= out.p[k] != nullptr;
     float *partial = columns ? (float *)a.workspace : nullptr;
-    const bool gate = a.x_codes ? a.gate_codes != nullptr : a.gate != nullptr;
-    const bool all = a.has_post && a.has_pre && a.dy && a.dh && a.dx && a.dbranch && (!gate || a.dgate);
-    const auto kernel = a.x_codes ? (!all ? norms_backward_kernel<DT, EV, CH, MULTI, 0, true> : gate ? norms_backward_kernel<DT, EV, CH, MULTI, 1, true>
-                                                                                                      : norms_backward_kernel<DT, EV, CH, MULTI, 2, true>)
-                                  : (!all ? norms_backward_kernel<DT, EV, CH, MULTI, 0, false> : gate ? norms_backward_kernel<DT, EV, CH, MULTI, 1, false>
-                                                                                                       : norms_backward_kernel<DT, EV, CH, MULTI, 2, false>);
+    const void *gate = a.x_codes ? a.gate_codes : a.gate;
+    using Kernel = void (*)(sn_block_norms_args, float *);
+    static constexpr Kernel kernels[2][8] = {SN_NORMS_MODES(norms_backward_kernel, false), SN_NORMS_MODES(norms_backward_kernel, true)};
+    const bool rest = a.dy && (a.dh || !a.has_pre) && a.dx && a.dbranch && (!gate || a.dgate);
+    const Kernel kernel = kernels[a.x_codes != nullptr][mode_of(a, gate, rest)];
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(MULTI ? waves_for(a.width) * 64 : 256), 0, st, a, partial);
     SN_CHECK_LAUNCH("sn_block_norms_backward");
     if (columns) {
