@@ -243,9 +243,9 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
 // MODE: 0 = the parts of the call are looked up at run time; otherwise the sum of those that are there: 1 the gate, 2 the norm after the
 // block, 4 the norm before the next one.  The branches of mode 0 make the compiler wait for all loads and stores in flight where it needs
 // the oldest row, the straight lines of the others do not (us, forward / backward, looked up and straight: bf16, 131072 rows of 1024, all
-// parts 268 / 464 and 263 / 408, both norms 253 / 410 and 216 / 312, the second alone 215 / 357 and 191 / 309, the first alone 180 / 327 and 141 / 242 (x is not read); 32768 rows of 4096, all
-// parts 326 / 464 and 306 / 418; fp32, 103424 rows of 256 118 / 162 and 108 / 161).  For the same reason rows that do not count are passed
-// over by scalar arithmetic, and get their zeros in a loop of their own.
+// parts 268 / 464 and 263 / 408, both norms 253 / 410 and 216 / 312, the second alone 215 / 357 and 191 / 309, the first alone 180 / 327
+// and 141 / 242 (x is not read); 32768 rows of 4096, all parts 326 / 464 and 306 / 418; fp32, 103424 rows of 256, all parts 118 / 162 and
+// 108 / 161).  For the same reason rows that do not count are passed over by scalar arithmetic, and get their zeros in a loop of their own.
 template <int DT, int EV, int CH, bool MULTI, int MODE, bool KEEP>
 __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block_norms_args a)
 {
