@@ -5,7 +5,8 @@ networks (`gated_residual_norms`), of activations kept in 8 bits for the backwar
 They take CUDA tensors in float32, bfloat16 or float16 with rows of any stride, compute in float32 and round each result
 once; outputs are new contiguous tensors; nothing synchronises, all of them can be captured into a graph.  Under `torch.autocast`
 their floating-point inputs are cast to float32, like those of the other HIP-backed ops of this package.  Arguments that do not
-fit raise RuntimeError before anything is launched.
+fit raise RuntimeError before anything is launched; tensors with a forward-mode tangent, which would be lost, raise
+NotImplementedError.
 
 Checks, buffers, launches and autograd nodes are C++ (csrc/sn_torch.cpp): a small call is bound by its host part."""
 import math
@@ -97,7 +98,8 @@ def checkpoint8_weight_grad(dy, kept, bias=True, out_dtype=None):
 
     dW = sum_r dy[r]^T kept[r] on the bf16 matrix cores with float32 sums.  The kept values are exact in bf16 and dy enters as
     bf16 pieces that add up to it (float32: three, float16: two), so the products carry no rounding of their own.  A gradient that is
-    infinite or NaN (float32: or beyond bfloat16's largest, 3.39e38) makes its feature's row of dW infinite or NaN.
+    infinite or NaN (float32: or beyond bfloat16's largest, 3.39e38) makes its feature's row of dW infinite or NaN.  No autograd: the
+    results carry no history of dy, and a dy with a forward-mode tangent is refused.
     out_dtype: the type of both results (default dy's)."""
     _need(isinstance(kept, Checkpoint8), "checkpoint8_weight_grad: expected a Checkpoint8, got {}", type(kept).__name__)
     return N.blocks().weight_grad(dy, kept._codes, kept._exps, kept._shape, bias, out_dtype)

@@ -10,6 +10,7 @@
 #include <stdexcept>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -79,6 +80,15 @@ void one_device(std::initializer_list<const Tensor *> tensors)
         else if (t->device() != first->device())
             refuse("tensors on different devices: %s vs %s", first->device().str().c_str(), t->device().str().c_str());
     }
+}
+
+// Forward-mode derivatives are not carried: the result of a tensor with a tangent would read as one whose tangent is zero.  (Inside a
+// Function's forward the mode is off, and the Function's own jvp answers for its inputs.)
+void no_tangents(std::initializer_list<const Tensor *> tensors, const char *who)
+{
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor *t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), who, ": no forward-mode derivatives");
 }
 
 void before_launch()
@@ -197,6 +207,7 @@ struct GatedResidualNormsBackward : torch::autograd::Node {
     variable_list apply(variable_list &&grads) override
     {
         std::lock_guard<std::mutex> lock(mutex_);
+        no_tangents({&grads.front(), &grads.back()}, "gated_residual_norms (backward)");
         variable_list out(8);
         {
             at::AutoDispatchBelowADInplaceOrView raw;
@@ -318,6 +329,7 @@ std::pair<Tensor, Tensor> gated_residual_norms(const Tensor &x, const Tensor &br
     const Tensor &v = c.n_valid;
     if (v.defined() && !(x.dim() == 3 && v.scalar_type() == at::kInt && v.dim() == 1 && v.size(0) == x.size(0) && v.is_contiguous()))
         refuse("gated_residual_norms: n_valid must be int32 [G] with x [G, n, width]");
+    no_tangents({&x, &branch, &gate, &p[0], &p[1], &p[2], &p[3], &p[4]}, "gated_residual_norms");
     one_device({&x, &branch, &gate, &v, &p[0], &p[1], &p[2], &p[3], &p[4]});
     for (Tensor &t : p)
         if (t.defined()) t = (mixed ? t.to(at::kFloat) : t).contiguous();
@@ -365,6 +377,7 @@ struct LabelLogProbsBackward : torch::autograd::Node {
     variable_list apply(variable_list &&grads) override
     {
         std::lock_guard<std::mutex> lock(mutex_);
+        no_tangents({&grads[0], &grads[1]}, "label_log_probs (backward)");
         variable_list out(1);
         if ((grads[0].defined() || grads[1].defined()) && task_should_compute_output(0)) {
             at::AutoDispatchBelowADInplaceOrView raw;
@@ -397,6 +410,7 @@ Scores label_log_probs(const Tensor &logits, const Tensor &given, int64_t topk, 
     if (n < 1 || n >= 1 << 30 || rows >= 1 << 24) refuse("label_log_probs: %lld rows of %lld entries", (long long)rows, (long long)n);
     if (topk < 0 || topk > n || topk > SN_SCORES_MAX_TOP)
         refuse("label_log_probs: %lld alternatives of %lld entries (at most %d)", (long long)topk, (long long)n, SN_SCORES_MAX_TOP);
+    no_tangents({&logits}, "label_log_probs");
     one_device({&logits, &given});
     std::shared_ptr<LabelLogProbsBackward> node;
     if (at::GradMode::is_enabled() && logits.requires_grad()) {
@@ -489,6 +503,7 @@ std::pair<Tensor, Tensor> weight_grad(const Tensor &dy, const Tensor &codes, con
     if (type_of(type) < 0) refuse("checkpoint8_weight_grad: cannot write %s", c10::toString(type));
     if (dy.dim() < 2 || dy.size(-1) < 1 || dy.sizes().slice(0, dy.dim() - 1) != shape.slice(0, shape.size() - 1))
         refuse("checkpoint8_weight_grad: gradients %s do not fit the activation %s", shown(dy.sizes()).c_str(), shown(shape).c_str());
+    no_tangents({&dy}, "checkpoint8_weight_grad");
     one_device({&dy, &codes, &exps});
     at::AutoDispatchBelowADInplaceOrView raw;
     const c10::DeviceGuard device(dy.device());
@@ -571,6 +586,8 @@ template <class F> PyObject *guarded(Py_ssize_t got, Py_ssize_t count, F body)
         if (got != count) refuse("expected %d arguments, got %d", (int)count, (int)got);
         return body();
     } catch (const PythonError &) {
+    } catch (const c10::NotImplementedError &e) {
+        PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
     } catch (const std::exception &e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     } catch (...) {

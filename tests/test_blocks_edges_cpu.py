@@ -1,0 +1,49 @@
+"""CPU (-m "not gpu"): calls of the operators of include/schemanet_blocks.h that have to be turned down before a launch: derivatives that
+would be lost, sizes past 32 bits.  No kernel is launched here."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import cpp_extension
+    cpp_extension.build()
+    from cpp_extension import ops
+    return ops
+
+
+def dual(*shape):
+    return fwd.make_dual(torch.ones(*shape), torch.ones(*shape))
+
+
+@pytest.mark.parametrize("name", ["x", "branch", "gate", "scale", "post weight", "post bias", "pre weight", "pre bias"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_norms_refuse_a_forward_mode_tangent(ops, name, grad):
+    v = {k: torch.ones(3, 8) for k in ("x", "branch", "gate")}
+    v.update({k: torch.ones(8) for k in ("scale", "post weight", "post bias", "pre weight", "pre bias")})
+    call = lambda: ops.gated_residual_norms(v["x"], v["branch"], gate=v["gate"], scale=v["scale"], post=(v["post weight"], v["post bias"]),      # noqa: E731
+                                            pre=(v["pre weight"], v["pre bias"]))
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        v[name] = dual(*v[name].shape)
+        with pytest.raises(NotImplementedError, match="gated_residual_norms: no forward-mode"):
+            call()
+        with fwd._set_fwd_grad_enabled(False):                       # inside a Function's forward: its jvp answers for its inputs
+            with pytest.raises(RuntimeError, match="no CPU fallback"):
+                call()
+
+
+def test_scores_refuse_a_forward_mode_tangent(ops):
+    target = torch.zeros(3, dtype=torch.int64)
+    with fwd.dual_level():
+        x = dual(3, 8)
+        with pytest.raises(NotImplementedError, match="label_log_probs: no forward-mode"):
+            ops.label_log_probs(x, target)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="label_log_probs: no forward-mode"):
+            ops.label_log_probs(x, target, topk=2)
+
+
+def test_weight_grad_refuses_a_forward_mode_tangent(ops):
+    kept = ops.Checkpoint8(torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 1, dtype=torch.uint8), (6, 20), torch.float32)
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="checkpoint8_weight_grad: no forward-mode"):
+        ops.checkpoint8_weight_grad(dual(6, 5), kept)
