@@ -31,7 +31,7 @@ int sn_blocks_abi_version(void);
  * codes [rows, npad] int8, exps [rows, npad / 32] uint8, npad = n rounded up to 32 (the codes beyond n are zero).
  * ------------------------------------------------------------------------------------------ */
 int sn_checkpoint8(const void *x, int dtype, int64_t rows, int n, int64_t row_stride, void *codes, void *exps, void *stream);
-/* out [rows, n] contiguous */
+/* out [rows, n] contiguous; SN_F16: kept values beyond 65504 come back as 65504 (8 bits round 65024 .. 65504 up to 65536) */
 int sn_checkpoint8_restore(const void *codes, const void *exps, int64_t rows, int n, void *out, int dtype, void *stream);
 
 /* dw [out_features, in_features] = sum_r dy[r, :]^T kept[r, :], db [out_features] = sum_r dy[r, :] (NULL: not wanted), kept =

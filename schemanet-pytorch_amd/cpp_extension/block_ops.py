@@ -81,7 +81,8 @@ class Checkpoint8:
         return self.codes.numel() + self.exps.numel()
 
     def restore(self, dtype=None):
-        """the kept values, [..., n] in `dtype` (default: the type of the activation; bfloat16 and float32 hold them exactly)"""
+        """the kept values, [..., n] in `dtype` (default: the type of the activation).  bfloat16 and float32 hold them exactly; float16 rounds
+        them and takes those beyond its largest to +-65504: 8 bits keep 65024 .. 65504 as 65536, and no finite activation comes back infinite"""
         return N.blocks().restore(self._codes, self._exps, self._shape, dtype or self.dtype)
 
 

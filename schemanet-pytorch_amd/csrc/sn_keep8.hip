@@ -56,6 +56,10 @@ __global__ __launch_bounds__(kPackThreads) void restore8_kernel(const uint8_t *c
         for (int k = 0; k < EV / 4; ++k) q[k] = src[k];
         float v[EV];
         decode<EV>(v, q, exps[r * (npad / 32) + j / 32]);
+        if constexpr (DT == SN_F16) {                        // a value from 65024 on was kept as 65536: to fp16's largest, not to infinity (NaN stays)
+#pragma unroll
+            for (int k = 0; k < EV; ++k) v[k] = fabsf(v[k]) > 65504.0f ? copysignf(65504.0f, v[k]) : v[k];
+        }
         store_row<DT, EV>((char *)out + r * n * (DT == SN_F32 ? 4 : 2), j, n, v);
     }
 }

@@ -1,4 +1,5 @@
-"""GPU tests of the operators of include/schemanet_blocks.h at their edges: derivatives that would be lost."""
+"""GPU tests of the operators of include/schemanet_blocks.h at their edges: derivatives that would be lost, values at
+the end of a type's range."""
 import os
 import sys
 
@@ -63,3 +64,24 @@ def test_function_transforms_are_refused(ops):
     for f in (lambda v: ops.gated_residual_norms(v, v)[0], lambda v: ops.checkpoint8(v).restore()):
         with pytest.raises(RuntimeError):
             torch.func.vmap(f)(x)
+
+
+# ------------------------------------------------------------------------------------------------ the end of a type's range
+@pytest.mark.parametrize("n", [1, 5, 8, 33, 256])
+def test_restore_to_float16_stays_finite(ops, n):
+    """float16 activations up to the largest: a block with max|x| >= 65280 has step 1024, so an element is off by at most 512, and
+    max|x| = 65504 -> 64 steps = 65536, which float16 does not have.  What was infinite or NaN marks its block as before."""
+    for top in (65504.0, 65472.0, 65024.0, 64992.0, 65280.0, 65248.0, 32768.0):
+        g = gen(int(top) + n)
+        x = (torch.rand(7, n, generator=g) * 2 - 1) * top
+        x[:, 0], x[3, 0] = top, -top
+        x = x.to(F16).to(DEV)
+        kept = ops.checkpoint8(x)
+        got, held = kept.restore(), kept.restore(F32)
+        assert got.dtype == F16 and torch.isfinite(got).all()
+        step = 1024.0 if top >= 65280.0 else 512.0 if top >= 32640.0 else 256.0
+        assert float((got.double() - x.double()).abs().max()) <= step / 2
+        assert torch.equal(got, held.clamp(-65504.0, 65504.0).to(F16))
+    wide = torch.tensor([[70000.0, -1e6, 1.0, 0.0], [3e38, -3e38, 0.0, 0.0], [float("inf"), 1.0, 2.0, 3.0], [1.0, float("nan"), 2.0, 3.0]], device=DEV)
+    got = ops.checkpoint8(wide).restore(F16)
+    assert got[0, :2].tolist() == [65504.0, -65504.0] and got[1].tolist() == [65504.0, -65504.0, 0.0, 0.0] and torch.isnan(got[2:]).all()
