@@ -53,12 +53,12 @@ template <bool MULTI> __device__ __forceinline__ void row_sum2(float &p, float &
 }
 
 // 1 / (1 + exp(-z)).  bf16 and fp16 rows: the hardware's 2^x of the rounded product (off by 2^-24 |z| relative, far under a step of
-// the result's type).  fp32 rows: with the product's rounding error as a first-order factor.
-template <int DT> __device__ __forceinline__ float sigmoid(float z)
+// the result's type).  fp32 rows: with the product's rounding error as a first-order factor.  e: exp(-z)
+template <int DT> __device__ __forceinline__ float sigmoid(float z, float &e)
 {
     constexpr float L = 1.44269504088896340736f, Llo = 1.92596299112661746887e-8f, ln2 = 0.693147180559945309f;
     const float t = -z * L;
-    float e = __builtin_amdgcn_exp2f(t);
+    e = __builtin_amdgcn_exp2f(t);
     if constexpr (DT == SN_F32) {
         const float lo = fmaf(-z, L, -t) - z * Llo;
         // (beyond 2^126 e may be infinite and the sigmoid is under 2^-126; under 2^-126 e no longer shows in 1 + e; an infinite z has no lo)
@@ -66,6 +66,24 @@ template <int DT> __device__ __forceinline__ float sigmoid(float z)
     }
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
+template <int DT> __device__ __forceinline__ float sigmoid(float z)
+{
+    float e;
+    return sigmoid<DT>(z, e);
+}
+// The backward pass needs s = sigmoid(z) and 1 - s, each to its own last bits: one register holds the smaller of the two, 1 - s = e s of
+// an open gate (z > 0) as it is, s of a closed one with its sign turned; the other is one subtraction from 1 that cannot cancel.  (1 - s
+// of a rounded s is off by 1e-3 of itself at z = 10 and zero from 17 on.)
+template <int DT> __device__ __forceinline__ float gate_parts(float z, float &s)
+{
+    float e;
+    s = sigmoid<DT>(z, e);
+    float w = z > 0.0f ? e * s : -s;
+    asm("" : "+v"(w));                       // (or the compiler keeps both in registers after all: 8 to 16 more, a wave less in places)
+    return w;
+}
+__device__ __forceinline__ float gate_opened(float w) { return __float_as_int(w) < 0 ? -w : 1.0f - w; }
+__device__ __forceinline__ float gate_closed(float w) { return __float_as_int(w) < 0 ? 1.0f + w : w; }
 
 template <int EV, int CH> struct Row { float v[CH][EV]; };
 
@@ -415,7 +433,7 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
         if (has_dh) take_cols<DT, EV, CH>(d, s.dh, col, step, E, tail);
         const float4 st = s.st;
         issue(s, after < a.rows ? after : row);
-        // f -> unit values of the post norm, z -> sigmoid, x -> unit values of y.  Columns beyond E hold whatever the statistics make of
+        // f -> unit values of the post norm, z -> the gate's parts, x -> unit values of y.  Columns beyond E hold whatever the statistics make of
         // zeros: every use multiplies it by a weight or a gradient that is zero there, and no store takes it.
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -424,8 +442,9 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
                 f.v[c][i] = (f.v[c][i] - st.x) * st.y;
                 float p = fmaf(f.v[c][i], w1.v[c][i], b1.v[c][i]);
                 if (gated) {
-                    z.v[c][i] = sigmoid<DT>(z.v[c][i]);
-                    p *= z.v[c][i];
+                    float open;
+                    z.v[c][i] = gate_parts<DT>(z.v[c][i], open);
+                    p *= open;
                 }
                 x.v[c][i] = (fmaf(p, sc.v[c][i], x.v[c][i]) - st.z) * st.w;
             }
@@ -457,10 +476,10 @@ __global__ __launch_bounds__(block_of(MULTI)) void norms_backward_kernel(sn_bloc
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
                 const float p = fmaf(f.v[c][i], w1.v[c][i], b1.v[c][i]);
-                const float us = gated ? u.v[c][i] * z.v[c][i] : u.v[c][i];
+                const float us = gated ? u.v[c][i] * gate_opened(z.v[c][i]) : u.v[c][i];
                 sum[2].v[c][i] = fmaf(us, p, sum[2].v[c][i]);
                 const float dp = us * sc.v[c][i];
-                if (gated) x.v[c][i] = dp * p * (1.0f - z.v[c][i]);
+                if (gated) x.v[c][i] = dp * p * gate_closed(z.v[c][i]);
                 sum[3].v[c][i] = fmaf(dp, f.v[c][i], sum[3].v[c][i]);
                 sum[4].v[c][i] += dp;
                 d.v[c][i] = dp * w1.v[c][i];

@@ -12,9 +12,13 @@ for p in (ROOT, os.path.join(ROOT, "schemanet-pytorch_amd"), os.path.join(ROOT, 
     if p not in sys.path:
         sys.path.insert(0, p)
 
+from blocks_plain import HALF, U, Norms64, check, kept64  # noqa: E402
+
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+K_ROW = 128                                       # roundings in a row of the norms' backward pass, as counted in test_gpu_blocks.py
+TINY = {F32: 2.0 ** -140, BF16: 2.0 ** -133, F16: 2.0 ** -24}
 
 
 @pytest.fixture(scope="module")
@@ -30,6 +34,10 @@ def gen(seed):
 
 def rand(g, *shape, dtype=F32, std=1.0, mean=0.0):
     return (torch.randn(*shape, generator=g) * std + mean).to(dtype).to(DEV)
+
+
+def d64(t):
+    return None if t is None else t.detach().double()
 
 
 # ------------------------------------------------------------------------------------------------ derivatives that would be lost
@@ -85,3 +93,42 @@ def test_restore_to_float16_stays_finite(ops, n):
     wide = torch.tensor([[70000.0, -1e6, 1.0, 0.0], [3e38, -3e38, 0.0, 0.0], [float("inf"), 1.0, 2.0, 3.0], [1.0, float("nan"), 2.0, 3.0]], device=DEV)
     got = ops.checkpoint8(wide).restore(F16)
     assert got[0, :2].tolist() == [65504.0, -65504.0] and got[1].tolist() == [65504.0, -65504.0, 0.0, 0.0] and torch.isnan(got[2:]).all()
+
+
+# ------------------------------------------------------------------------------------------------ gates far open and far closed
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("width", [3, 200, 300, 1100])
+def test_gradient_of_open_and_closed_gates(ops, dtype, width, keep8):
+    """dgate = dy scale branch s (1 - s) without norms: each factor has its own relative error, 1 - s of an open gate among them.  The
+    roundings: the exponent's product |z| U twice, exp 2, sum, reciprocal 2, e s, four products: (16 + 2 |z|) U of the value."""
+    g = gen(width)
+    z = (torch.rand(9, width, generator=g) * 60 - 30).to(dtype)
+    z[0], z[1], z[2], z[3] = 17.5, 30.0, -30.0, 0.0
+    z = z.to(DEV).requires_grad_()
+    x, f, dy, scale = rand(g, 9, width, dtype=dtype), rand(g, 9, width, dtype=dtype, std=20.0), rand(g, 9, width, dtype=dtype, std=50.0), rand(g, width, dtype=dtype)
+    y, _ = ops.gated_residual_norms(x, f, gate=z, scale=scale, checkpoint8=keep8)
+    got, = torch.autograd.grad(y, z, dy)
+    zz, ff = (kept64(d64(z)), kept64(d64(f))) if keep8 else (d64(z), d64(f))
+    want = d64(dy) * d64(scale) * ff * torch.sigmoid(zz) * torch.sigmoid(-zz)
+    check(got, want, HALF[dtype] * want.abs() + (16 + 2 * zz.abs()) * U * want.abs() * (1 + HALF[dtype]) + TINY[dtype], "dgate")
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("dtype,width", [(F32, 256), (F32, 700), (BF16, 128), (BF16, 2000)])
+def test_gradient_of_open_gates_between_norms(ops, dtype, width, norm, keep8):
+    """the same between both norms: K_ROW roundings of the formula with absolute values, s (1 - s) in it"""
+    g = gen(width)
+    shape = (33, width)
+    z = (torch.rand(*shape, generator=g) * 22 + 8).to(dtype).to(DEV).requires_grad_()
+    x, f, dy, dh = (rand(g, *shape, dtype=dtype, std=s) for s in (2.0, 1.0, 30.0, 30.0))
+    scale, w1, b1, w2, b2 = (rand(g, width, dtype=dtype, std=0.3, mean=m) for m in (1.0, 1.0, 0.0, 1.0, 0.0))
+    y, h = ops.gated_residual_norms(x, f, gate=z, scale=scale, post=(w1, b1), pre=(w2, b2), norm=norm, checkpoint8=keep8)
+    got, = torch.autograd.grad([y, h], z, [dy, dh])
+    kept = tuple(kept64(d64(t)) for t in (x, f, z)) if keep8 else None
+    r = Norms64(d64(x), d64(f), d64(z), d64(scale), (d64(w1), d64(b1)), (d64(w2), d64(b2)), norm, 1e-5, d64(dy), d64(dh), kept)
+    zz = kept[2] if keep8 else d64(z)
+    closed = torch.sigmoid(-zz)
+    want = r.dgate / (1 - torch.sigmoid(zz)) * closed               # (the definition's own 1 - s cancels in 64 bits too, by 1e-3 at 30)
+    check(got, want, HALF[dtype] * want.abs() + (K_ROW + 2 * zz.abs()) * U * r.dgate_mag * closed * (1 + HALF[dtype]) + TINY[dtype], "dgate")
