@@ -457,6 +457,9 @@ Scores label_log_probs(const Tensor &logits, const Tensor &given, int64_t topk, 
 }
 
 // ------------------------------------------------------------------------------------------------------- 8-bit checkpoints
+// the entry points' own limits, tested here too: they see the numbers as 32-bit ones
+constexpr int64_t kMostFeatures = 1 << 30, kMostProduct = 1 << 20;
+
 int64_t rows_in(at::IntArrayRef shape)
 {
     int64_t rows = 1;
@@ -468,6 +471,7 @@ std::pair<Tensor, Tensor> checkpoint8(const Tensor &x)
 {
     if (!x.defined() || type_of(x) < 0) refuse("checkpoint8: expected a float32, bfloat16 or float16 tensor");
     if (x.dim() < 1 || x.size(-1) < 1) refuse("checkpoint8: expected at least one feature, got shape %s", shown(x.sizes()).c_str());
+    if (x.size(-1) > kMostFeatures) refuse("checkpoint8: %lld features (at most 2^30)", (long long)x.size(-1));
     one_device({&x});
     at::AutoDispatchBelowADInplaceOrView raw;
     const c10::DeviceGuard device(x.device());
@@ -484,6 +488,7 @@ std::pair<Tensor, Tensor> checkpoint8(const Tensor &x)
 Tensor restore(const Tensor &codes, const Tensor &exps, at::IntArrayRef shape, at::ScalarType type)
 {
     if (type_of(type) < 0) refuse("checkpoint8: cannot restore to %s", c10::toString(type));
+    if (shape.back() > kMostFeatures) refuse("checkpoint8: %lld features (at most 2^30)", (long long)shape.back());
     one_device({&codes, &exps});
     at::AutoDispatchBelowADInplaceOrView raw;
     const c10::DeviceGuard device(codes.device());
@@ -503,6 +508,8 @@ std::pair<Tensor, Tensor> weight_grad(const Tensor &dy, const Tensor &codes, con
     if (type_of(type) < 0) refuse("checkpoint8_weight_grad: cannot write %s", c10::toString(type));
     if (dy.dim() < 2 || dy.size(-1) < 1 || dy.sizes().slice(0, dy.dim() - 1) != shape.slice(0, shape.size() - 1))
         refuse("checkpoint8_weight_grad: gradients %s do not fit the activation %s", shown(dy.sizes()).c_str(), shown(shape).c_str());
+    if (dy.size(-1) > kMostProduct || shape.back() > kMostProduct)
+        refuse("checkpoint8_weight_grad: %lld x %lld features (at most 2^20 each)", (long long)dy.size(-1), (long long)shape.back());
     no_tangents({&dy}, "checkpoint8_weight_grad");
     one_device({&dy, &codes, &exps});
     at::AutoDispatchBelowADInplaceOrView raw;

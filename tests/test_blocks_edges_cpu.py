@@ -47,3 +47,23 @@ def test_weight_grad_refuses_a_forward_mode_tangent(ops):
     kept = ops.Checkpoint8(torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 1, dtype=torch.uint8), (6, 20), torch.float32)
     with fwd.dual_level(), pytest.raises(NotImplementedError, match="checkpoint8_weight_grad: no forward-mode"):
         ops.checkpoint8_weight_grad(dual(6, 5), kept)
+
+
+@pytest.mark.parametrize("n", [(1 << 30) + 1, 1 << 31, (1 << 32) + 32])
+def test_features_past_32_bits_are_refused(ops, n):
+    """2^32 + 32 features read as 32 would leave most of the checkpoint unwritten.  (Views of one element: no memory.)"""
+    with pytest.raises(RuntimeError, match="features"):
+        ops.checkpoint8(torch.zeros(1).expand(n))
+    with pytest.raises(RuntimeError, match="features"):
+        ops.checkpoint8(torch.zeros(1, 1, dtype=torch.bfloat16).expand(2, n))
+    npad = (n + 31) // 32 * 32
+    kept = ops.Checkpoint8(torch.zeros(0, npad, dtype=torch.int8), torch.zeros(0, npad // 32, dtype=torch.uint8), (0, n), torch.float32)
+    with pytest.raises(RuntimeError, match="features"):
+        kept.restore()
+    with pytest.raises(RuntimeError, match="features"):
+        ops.checkpoint8_weight_grad(torch.zeros(0, 4), kept)
+    few = ops.Checkpoint8(torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 1, dtype=torch.uint8), (6, 20), torch.float32)
+    with pytest.raises(RuntimeError, match="features"):
+        ops.checkpoint8_weight_grad(torch.zeros(1, 1).expand(6, n), few)
+    with pytest.raises(RuntimeError, match="features"):
+        ops.checkpoint8_weight_grad(torch.zeros(1, 1).expand(6, (1 << 20) + 1), few)
