@@ -329,6 +329,7 @@ std::pair<Tensor, Tensor> gated_residual_norms(const Tensor &x, const Tensor &br
     const Tensor &v = c.n_valid;
     if (v.defined() && !(x.dim() == 3 && v.scalar_type() == at::kInt && v.dim() == 1 && v.size(0) == x.size(0) && v.is_contiguous()))
         refuse("gated_residual_norms: n_valid must be int32 [G] with x [G, n, width]");
+    if (v.defined() && x.size(1) > INT32_MAX) refuse("gated_residual_norms: %lld vertices a graph (under 2^31 with n_valid)", (long long)x.size(1));
     no_tangents({&x, &branch, &gate, &p[0], &p[1], &p[2], &p[3], &p[4]}, "gated_residual_norms");
     one_device({&x, &branch, &gate, &v, &p[0], &p[1], &p[2], &p[3], &p[4]});
     for (Tensor &t : p)

@@ -67,3 +67,13 @@ def test_features_past_32_bits_are_refused(ops, n):
         ops.checkpoint8_weight_grad(torch.zeros(1, 1).expand(6, n), few)
     with pytest.raises(RuntimeError, match="features"):
         ops.checkpoint8_weight_grad(torch.zeros(1, 1).expand(6, (1 << 20) + 1), few)
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 1])
+def test_vertices_past_32_bits_are_refused(ops, n):
+    """2^32 + 1 vertices of one graph read as 1 would take every vertex for a graph with an extent of its own.  (Views: no memory.)"""
+    x = torch.zeros(1, 1, 1).expand(1, n, 1)
+    with pytest.raises(RuntimeError, match="vertices"):
+        ops.gated_residual_norms(x, x, n_valid=torch.ones(1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.gated_residual_norms(x, x)
