@@ -1005,7 +1005,8 @@ class _EdgesAdjMatmul(torch.autograd.Function):
         ext = adj_planes.compact[1] if adj_planes.compact is not None else None      # compacted class graphs: one extent per graph
         xt = split_planes(x.detach(), transpose=True, node_extents=ext)
         y = gcn_gemm(adj_planes, xt, G, want_c=True, zero_c=ext is not None, m_extent=ext, k_extent=ext, rows_valid=ext)["c"]
-        ctx.save_for_backward(x)
+        if ctx.needs_input_grad[0]:                          # (only the edges' gradient reads X)
+            ctx.save_for_backward(x)
         ctx.adj_planes = adj_planes
         ctx.x_scale = xt.scale                               # (the backward's planes of x: no second reduction over it)
         ctx.adj_like = torch.empty(edges.shape, dtype=edges.dtype, device="meta")
@@ -1017,13 +1018,13 @@ class _EdgesAdjMatmul(torch.autograd.Function):
     @staticmethod
     @_amp_bwd
     def backward(ctx, dy):
-        (x,) = ctx.saved_tensors
+        saved = ctx.saved_tensors
         ap = ctx.adj_planes
-        G = x.shape[0]
         dy = _f32c(dy)
+        G = dy.shape[0]
         if dy.numel() == 0:
-            return (torch.zeros(ctx.adj_like.shape, dtype=ctx.adj_like.dtype, device=x.device) if ctx.needs_input_grad[0] else None,
-                    torch.zeros_like(x) if ctx.needs_input_grad[1] else None, None, None)
+            return (torch.zeros(ctx.adj_like.shape, dtype=ctx.adj_like.dtype, device=dy.device) if ctx.needs_input_grad[0] else None,
+                    torch.zeros_like(dy) if ctx.needs_input_grad[1] else None, None, None)
         d_e = d_x = None
         dy_scale = pow2_scale(dy)                            # one reduction over dy for both of its plane forms
         ext = ap.compact[1] if ap.compact is not None else None
@@ -1031,7 +1032,7 @@ class _EdgesAdjMatmul(torch.autograd.Function):
             d_x = gcn_gemm(ap, split_planes(dy, scale=dy_scale, transpose=True, node_extents=ext), G, want_c=True, zero_c=ext is not None, m_extent=ext, k_extent=ext,
                            rows_valid=ext)["c"]
         if ctx.needs_input_grad[0]:
-            dyp, xp = split_planes(dy, scale=dy_scale, node_extents=ext), split_planes(x.detach(), scale=ctx.x_scale, node_extents=ext)
+            dyp, xp = split_planes(dy, scale=dy_scale, node_extents=ext), split_planes(saved[0].detach(), scale=ctx.x_scale, node_extents=ext)
             if not ctx.counted:
                 s_ = gcn_gemm(dyp, xp, G, want_c=True, m_extent=ext)["c"]
                 return _edge_grad_of(s_, ap), d_x, None, None

@@ -1,5 +1,5 @@
 """GPU tests of the operators of include/schemanet_blocks.h at their edges: derivatives that would be lost, values at
-the end of a type's range."""
+the end of a type's range, gates far open, and what a block with 8-bit checkpoints holds in memory."""
 import os
 import sys
 
@@ -132,3 +132,98 @@ def test_gradient_of_open_gates_between_norms(ops, dtype, width, norm, keep8):
     closed = torch.sigmoid(-zz)
     want = r.dgate / (1 - torch.sigmoid(zz)) * closed               # (the definition's own 1 - s cancels in 64 bits too, by 1e-3 at 30)
     check(got, want, HALF[dtype] * want.abs() + (K_ROW + 2 * zz.abs()) * U * r.dgate_mag * closed * (1 + HALF[dtype]) + TINY[dtype], "dgate")
+
+
+# ------------------------------------------------------------------------------------------------ what a block holds
+def residual_gnn(activation, layers, checkpoint8, E=256):
+    import schema_inference.graph as graph
+    torch.manual_seed(7)
+    gnn = graph.GNN(50, E, layers, activation=activation, residual=True, checkpoint8=checkpoint8).to(DEV)
+    with torch.no_grad():
+        for layer in gnn.layers:
+            layer.scale.add_(0.5)
+    return gnn
+
+
+def graphs(G=4, n=192, edge_grad=False):
+    g = gen(5)
+    return dict(nodes=torch.rand(G, n, generator=g).to(DEV), edges=(torch.rand(G, n, n, generator=g) / n).to(DEV).requires_grad_(edge_grad),
+                ingredients=torch.randint(0, 50, (G, n), generator=g).to(DEV), n_valid=torch.tensor([192, 3, 100, 191], dtype=torch.int32, device=DEV),
+                divisor=torch.tensor([n], dtype=torch.int32, device=DEV))
+
+
+def held(gnn, data):
+    before = torch.cuda.memory_allocated(DEV)
+    out = gnn(**data)
+    return torch.cuda.memory_allocated(DEV) - before, out
+
+
+@pytest.mark.parametrize("edge_grad", [False, True])
+@pytest.mark.parametrize("activation,checkpoint8,whole,bytes8", [("relu", True, 0, 6), ("swish", True, 1, 5), ("none", True, 0, 5), ("relu", False, 5, 0), ("swish", False, 6, 0)])
+def test_what_a_block_holds(ops, activation, checkpoint8, whole, bytes8, edge_grad):
+    """bytes of one more block, by the allocator.  whole: float32 tensors; bytes8: those of one byte an element, all with their 1 / 32 of
+    exponents but for ReLU's signs.  Without checkpoints h and the Linear's input are among the whole ones and a gradient for the edges
+    adds none; with them it adds h and takes its checkpoint away.  Beside them 16 bytes of statistics a row and, for each allocation,
+    rounding up to 512 bytes."""
+    data = graphs(edge_grad=edge_grad)
+    some, more = residual_gnn(activation, 2, checkpoint8), residual_gnn(activation, 3, checkpoint8)
+    for gnn in (some, more):
+        gnn(**data)                                                   # (what is built once and kept)
+    a, out = held(some, data)
+    del out
+    b, out = held(more, data)
+    elements = 4 * 192 * 256
+    if checkpoint8 and edge_grad:
+        whole, bytes8 = whole + 1, bytes8 - 1
+    signs = 1 if checkpoint8 and activation == "relu" else 0
+    want = elements * (4 * whole + signs + (bytes8 - signs) * 33 / 32) + 16 * 4 * 192
+    assert want <= b - a <= want + 16 * 512, (b - a) / elements
+    torch.autograd.grad(out.sum(), list(more.parameters()))
+
+
+@pytest.mark.parametrize("activation", ["relu", "swish", "none"])
+@pytest.mark.parametrize("edge_grad", [False, True])
+def test_a_block_that_holds_less_computes_the_same(ops, activation, edge_grad):
+    """the forward pass is that of the block without checkpoints; gradients, those of the edges among them, differ by what 8 bits round:
+    each kept element by at most 1 / 127.5 of its block's maximum, uniformly distributed, so by under a tenth of a gradient's norm"""
+    data = graphs(edge_grad=edge_grad)
+    plain, kept = residual_gnn(activation, 3, False), residual_gnn(activation, 3, True)
+    kept.load_state_dict(plain.state_dict())
+    up = rand(gen(9), 4, 256)
+    results = []
+    for gnn in (plain, kept):
+        out = gnn(**data)
+        leaves = list(gnn.parameters()) + ([data["edges"]] if edge_grad else [])
+        results.append((out.detach(), torch.autograd.grad(out, leaves, up)))
+    assert torch.equal(results[0][0], results[1][0])
+    for a, b in zip(results[1][1], results[0][1]):
+        assert float((a.double() - b.double()).norm()) <= 0.1 * float(b.double().norm())
+
+
+def test_relu_of_signs_is_relu(ops):
+    from schema_inference.graph.gnn import _ReluOfSigns
+    x = rand(gen(11), 1000)
+    x[:6] = torch.tensor([0.0, -0.0, float("inf"), float("-inf"), float("nan"), 1e-45], device=DEV)
+    up = rand(gen(12), 1000)
+    got, want = [], []
+    for f, into in ((_ReluOfSigns.apply, got), (torch.relu, want)):
+        leaf = x.clone().requires_grad_()
+        y = f(leaf)
+        into += [y.detach(), torch.autograd.grad(y, leaf, up)[0]]
+    for a, b in zip(got, want):
+        assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) and torch.equal(a.isnan(), b.isnan())
+
+
+def test_the_adjacency_product_keeps_its_operand_for_the_edges_only(ops):
+    x = rand(gen(13), 3, 40, 64).requires_grad_()
+    for edge_grad in (False, True):
+        edges = rand(gen(14), 3, 40, 40).requires_grad_(edge_grad)
+        seen = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.shape) or t, lambda t: t):
+            y = ops.edges_adj_matmul(edges, x)
+        assert len(seen) == int(edge_grad)
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+        adj = (d64(edges) + d64(edges).transpose(1, 2)) / 2 + torch.eye(40, dtype=torch.float64, device=DEV)
+        want = adj.sum(1, keepdim=True).transpose(1, 2).expand(3, 40, 64)
+        # split-fp16 products are off by 2^-22 of an operand's largest magnitude for each of the 40 terms
+        assert float((dx.double() - want).abs().max()) <= 2.0 ** -22 * 40 * 2 * float(adj.abs().max())
