@@ -15,6 +15,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -46,8 +47,6 @@ struct Library {
 } lib;
 constexpr Py_ssize_t kEntries = sizeof(Library) / sizeof(void *);
 PyObject *require_gpu = nullptr;             // called before the first launch, then dropped
-
-struct PythonError {};                       // a Python exception is set
 
 [[noreturn]] void refuse(const char *format, ...)
 {
@@ -95,7 +94,7 @@ void before_launch()
 {
     if (!require_gpu) return;
     PyObject *r = PyObject_CallNoArgs(require_gpu);
-    if (!r) throw PythonError();
+    if (!r) throw python_error();
     Py_DECREF(r);
     Py_CLEAR(require_gpu);
 }
@@ -545,13 +544,13 @@ PyObject *python(const Tensor &t)
 {
     if (!t.defined()) Py_RETURN_NONE;
     PyObject *o = THPVariable_Wrap(t);
-    if (!o) throw PythonError();
+    if (!o) throw python_error();
     return o;
 }
 template <class... T> PyObject *python_tuple(const T &...ts)
 {
     PyObject *all = PyTuple_New(sizeof...(ts));
-    if (!all) throw PythonError();
+    if (!all) throw python_error();
     Py_ssize_t i = 0;
     try {
         (PyTuple_SET_ITEM(all, i++, python(ts)), ...);
@@ -564,13 +563,13 @@ template <class... T> PyObject *python_tuple(const T &...ts)
 int64_t integer(PyObject *o)
 {
     const long long v = PyLong_AsLongLong(o);
-    if (v == -1 && PyErr_Occurred()) throw PythonError();
+    if (v == -1 && PyErr_Occurred()) throw python_error();
     return v;
 }
 bool truth(PyObject *o)
 {
     const int v = PyObject_IsTrue(o);
-    if (v < 0) throw PythonError();
+    if (v < 0) throw python_error();
     return v != 0;
 }
 std::vector<int64_t> sizes(PyObject *o)
@@ -587,21 +586,14 @@ std::optional<at::ScalarType> scalar_type(PyObject *o)
     return reinterpret_cast<THPDtype *>(o)->scalar_type;
 }
 
-// (count: what the Python side passes; C++ exceptions end here)
+// (count: what the Python side passes; C++ exceptions end here, each as the Python one that torch makes of it: torch.OutOfMemoryError,
+// whatever a hook for saved tensors raised, NotImplementedError, RuntimeError)
 template <class F> PyObject *guarded(Py_ssize_t got, Py_ssize_t count, F body)
 {
-    try {
-        if (got != count) refuse("expected %d arguments, got %d", (int)count, (int)got);
-        return body();
-    } catch (const PythonError &) {
-    } catch (const c10::NotImplementedError &e) {
-        PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
-    } catch (const std::exception &e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-    } catch (...) {
-        PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
-    }
-    return nullptr;
+    HANDLE_TH_ERRORS
+    if (got != count) refuse("expected %d arguments, got %d", (int)count, (int)got);
+    return body();
+    END_HANDLE_TH_ERRORS
 }
 
 PyObject *py_norms(PyObject *, PyObject *const *a, Py_ssize_t n)
@@ -611,7 +603,7 @@ PyObject *py_norms(PyObject *, PyObject *const *a, Py_ssize_t n)
         NormsCall c;
         c.rms = truth(a[8]);
         const double eps = PyFloat_AsDouble(a[9]);
-        if (eps == -1.0 && PyErr_Occurred()) throw PythonError();
+        if (eps == -1.0 && PyErr_Occurred()) throw python_error();
         c.eps = (float)eps;
         c.n_valid = tensor(a[10], "gated_residual_norms: n_valid must be int32 [G] with x [G, n, width]");
         for (int i = 0; i < 5; ++i) c.params[i] = tensor(a[3 + i], parameters);

@@ -1,5 +1,5 @@
 """GPU tests of the operators of include/schemanet_blocks.h at their edges: derivatives that would be lost, values at
-the end of a type's range, gates far open, and what a block with 8-bit checkpoints holds in memory."""
+the end of a type's range, gates far open, what a block with 8-bit checkpoints holds in memory, and errors from below."""
 import os
 import sys
 
@@ -227,3 +227,40 @@ def test_the_adjacency_product_keeps_its_operand_for_the_edges_only(ops):
         want = adj.sum(1, keepdim=True).transpose(1, 2).expand(3, 40, 64)
         # split-fp16 products are off by 2^-22 of an operand's largest magnitude for each of the 40 terms
         assert float((dx.double() - want).abs().max()) <= 2.0 ** -22 * 40 * 2 * float(adj.abs().max())
+
+
+# ------------------------------------------------------------------------------------------------ errors from below
+def test_out_of_memory_is_torch_s(ops):
+    """4 TiB and more, which no card has: the allocator says so at once.  (Views of a few elements.)"""
+    x = torch.zeros(1, 1, device=DEV).expand(1 << 20, 1 << 20)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.checkpoint8(x)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.label_log_probs(x, torch.zeros(1 << 20, dtype=torch.int64, device=DEV))
+    narrow = torch.zeros(1, 1, device=DEV).expand(1 << 30, 4096)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.gated_residual_norms(narrow, narrow)
+    x = rand(gen(1), 4, 64)
+    assert torch.equal(ops.gated_residual_norms(x, x)[0], x + x)
+
+
+def test_hooks_for_saved_tensors_raise_their_own(ops):
+    x, target = rand(gen(2), 4, 64).requires_grad_(), torch.arange(4, device=DEV)
+
+    class Full(Exception):
+        pass
+
+    def raises(t):
+        raise Full("no room for " + str(tuple(t.shape)))
+    for call in (lambda: ops.gated_residual_norms(x, x), lambda: ops.gated_residual_norms(x, x, checkpoint8=True), lambda: ops.label_log_probs(x, target)):
+        with pytest.raises(Full, match="no room"):
+            with torch.autograd.graph.saved_tensors_hooks(raises, lambda t: t):
+                call()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, raises):
+            out = call()[0]
+        with pytest.raises(Full, match="no room"):
+            out.sum().backward()
+    with pytest.raises(RuntimeError, match="width 4097"):
+        ops.gated_residual_norms(torch.zeros(1, 4097, device=DEV), torch.zeros(1, 4097, device=DEV))
+    with pytest.raises(TypeError):
+        ops.gated_residual_norms(x, x, eps="small")
