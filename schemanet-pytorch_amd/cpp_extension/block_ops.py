@@ -48,7 +48,7 @@ class Checkpoint8:
     __slots__ = ("_codes", "_exps", "_shape", "dtype")
 
     def __init__(self, codes, exps, shape, dtype):
-        # (checked here, once: the kernels read both by the shape, and none of the three can be replaced later)
+        # (none of the three can be replaced later; what happens to the tensors in place is checked at each use)
         shape = tuple(shape)
         _need(len(shape) >= 1 and shape[-1] >= 1, "checkpoint8: expected at least one feature, got shape {}", shape)
         rows, npad = math.prod(shape[:-1]), (shape[-1] + 31) // 32 * 32

@@ -467,6 +467,19 @@ int64_t rows_in(at::IntArrayRef shape)
     return rows;
 }
 
+// The kernels read codes and exponents by the activation's shape.  Checked at each use: either may have been resized or freed in place
+// since the checkpoint was made, or come back from a hook for saved tensors.
+void check_kept(const Tensor &codes, const Tensor &exps, at::IntArrayRef shape)
+{
+    const int64_t rows = rows_in(shape), npad = (shape.back() + 31) / 32 * 32;
+    auto fits = [&](const Tensor &t, at::ScalarType type, int64_t columns) {
+        return t.defined() && t.scalar_type() == type && t.dim() == 2 && t.size(0) == rows && t.size(1) == columns && t.is_contiguous() &&
+               (int64_t)t.storage().nbytes() >= t.storage_offset() + rows * columns;
+    };
+    if (!fits(codes, at::kChar, npad) || !fits(exps, at::kByte, npad / 32))
+        refuse("checkpoint8: codes and exponents do not hold an activation %s (any more)", shown(shape).c_str());
+}
+
 std::pair<Tensor, Tensor> checkpoint8(const Tensor &x)
 {
     if (!x.defined() || type_of(x) < 0) refuse("checkpoint8: expected a float32, bfloat16 or float16 tensor");
@@ -489,6 +502,7 @@ Tensor restore(const Tensor &codes, const Tensor &exps, at::IntArrayRef shape, a
 {
     if (type_of(type) < 0) refuse("checkpoint8: cannot restore to %s", c10::toString(type));
     if (shape.back() > kMostFeatures) refuse("checkpoint8: %lld features (at most 2^30)", (long long)shape.back());
+    check_kept(codes, exps, shape);
     one_device({&codes, &exps});
     at::AutoDispatchBelowADInplaceOrView raw;
     const c10::DeviceGuard device(codes.device());
@@ -510,6 +524,7 @@ std::pair<Tensor, Tensor> weight_grad(const Tensor &dy, const Tensor &codes, con
         refuse("checkpoint8_weight_grad: gradients %s do not fit the activation %s", shown(dy.sizes()).c_str(), shown(shape).c_str());
     if (dy.size(-1) > kMostProduct || shape.back() > kMostProduct)
         refuse("checkpoint8_weight_grad: %lld x %lld features (at most 2^20 each)", (long long)dy.size(-1), (long long)shape.back());
+    check_kept(codes, exps, shape);
     no_tangents({&dy}, "checkpoint8_weight_grad");
     one_device({&dy, &codes, &exps});
     at::AutoDispatchBelowADInplaceOrView raw;

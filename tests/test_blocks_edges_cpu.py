@@ -1,5 +1,5 @@
 """CPU (-m "not gpu"): calls of the operators of include/schemanet_blocks.h that have to be turned down before a launch: derivatives that
-would be lost, sizes past 32 bits.  No kernel is launched here."""
+would be lost, sizes past 32 bits, checkpoints that no longer hold their activation.  No kernel is launched here."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -77,3 +77,19 @@ def test_vertices_past_32_bits_are_refused(ops, n):
         ops.gated_residual_norms(x, x, n_valid=torch.ones(1, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.gated_residual_norms(x, x)
+
+
+@pytest.mark.parametrize("change", [lambda k: k.codes.resize_(3, 32), lambda k: k.exps.resize_(0), lambda k: k.codes.t_(), lambda k: k.exps.t_(),
+                                    lambda k: k.codes.untyped_storage().resize_(0), lambda k: k.exps.untyped_storage().resize_(5),
+                                    lambda k: k.codes.unsqueeze_(0), lambda k: k.codes.as_strided_((6, 32), (1, 1)),
+                                    lambda k: setattr(k.codes, "data", torch.zeros(6, 16, dtype=torch.int8))])
+def test_a_checkpoint8_changed_in_place_is_refused(ops, change):
+    """the kernels read both buffers by the activation's shape: out of range, once they are smaller"""
+    kept = ops.Checkpoint8(torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6, 1, dtype=torch.uint8), (2, 3, 20), torch.float32)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        kept.restore()
+    change(kept)
+    with pytest.raises(RuntimeError, match="do not hold"):
+        kept.restore()
+    with pytest.raises(RuntimeError, match="do not hold"):
+        ops.checkpoint8_weight_grad(torch.zeros(2, 3, 4), kept)
