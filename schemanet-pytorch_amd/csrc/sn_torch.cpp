@@ -125,6 +125,42 @@ Rows rows_of(const Tensor &t, int64_t width)
     return {t, stride < 0 ? width : stride};
 }
 
+int64_t rows_in(at::IntArrayRef shape)
+{
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
+    return rows;
+}
+
+// The kernels read codes and exponents by the activation's shape.  Checked at each use: either may have been resized or freed in place
+// since the checkpoint was made, or come back from a hook for saved tensors.
+void check_kept(const Tensor &codes, const Tensor &exps, at::IntArrayRef shape)
+{
+    const int64_t rows = rows_in(shape), npad = (shape.back() + 31) / 32 * 32;
+    auto fits = [&](const Tensor &t, at::ScalarType type, int64_t columns) {
+        return t.defined() && t.scalar_type() == type && t.dim() == 2 && t.size(0) == rows && t.size(1) == columns && t.is_contiguous() &&
+               (int64_t)t.storage().nbytes() >= t.storage_offset() + rows * columns;
+    };
+    if (!fits(codes, at::kChar, npad) || !fits(exps, at::kByte, npad / 32))
+        refuse("checkpoint8: codes and exponents do not hold an activation %s (any more)", shown(shape).c_str());
+}
+
+// What a node saved (undefined if there was nothing), as it comes back: hooks for saved tensors may hand over anything, and the kernels
+// read it by the forward call's types and sizes.
+Tensor unpack(const SavedVariable &v, at::ScalarType type, at::IntArrayRef sizes, c10::Device device, const char *who)
+{
+    Tensor t = v.unpack();
+    if (t.defined() && (t.scalar_type() != type || t.sizes() != sizes || t.device() != device))
+        refuse("%s: a saved tensor of type %s and shape %s on %s came back as %s, %s on %s", who, c10::toString(type), shown(sizes).c_str(), device.str().c_str(),
+               c10::toString(t.scalar_type()), shown(t.sizes()).c_str(), t.device().str().c_str());
+    return t;
+}
+Tensor unpack_whole(const SavedVariable &v, at::ScalarType type, at::IntArrayRef sizes, c10::Device device, const char *who)
+{
+    const Tensor t = unpack(v, type, sizes, device, who);
+    return t.defined() ? t.contiguous() : t;
+}
+
 // A backward pass captured into a graph must not reach autograd nodes of the default stream, which cannot take part in a capture: those
 // that an eager graph of the same leaves keeps alive.  The engine would find out on its own thread and end the process.
 void before_capture(const torch::autograd::edge_list &edges, const char *who)
@@ -189,8 +225,9 @@ sn_block_norms_args norms_args(const NormsCall &c, int type, at::IntArrayRef sha
 
 struct GatedResidualNormsBackward : torch::autograd::Node {
     SavedVariable params[5], n_valid, stats, held[6];        // held: x, branch, gate or their checkpoints (codes, exps)
-    std::vector<int64_t> shape;
+    at::DimVector shape;
     at::TensorOptions options;
+    at::ScalarType param_type = at::kFloat;
     bool rms = false, kept = false, gated = false, empty_rows = false;
     float eps = 0;
 
@@ -218,8 +255,11 @@ struct GatedResidualNormsBackward : torch::autograd::Node {
     void run(const Tensor &dy, const Tensor &dh, variable_list &out)
     {
         if (!dy.defined() && !dh.defined()) return;
-        NormsCall c = {rms, eps, n_valid.unpack(), {}};
-        for (int i = 0; i < 5; ++i) c.params[i] = params[i].unpack();
+        const char *const who = "gated_residual_norms (backward)";
+        const c10::Device place = options.device();
+        const int64_t rows = rows_in(shape), width = shape.back();
+        NormsCall c = {rms, eps, unpack_whole(n_valid, at::kInt, at::IntArrayRef(shape).slice(0, 1), place, who), {}};
+        for (int i = 0; i < 5; ++i) c.params[i] = unpack_whole(params[i], param_type, width, place, who);
         bool want[8], columns = false;
         for (int i = 0; i < 8; ++i) want[i] = task_should_compute_output(i);
         want[2] = want[2] && gated;
@@ -230,10 +270,17 @@ struct GatedResidualNormsBackward : torch::autograd::Node {
                 if (want[3 + i] && c.params[i].defined()) out[3 + i] = at::zeros_like(c.params[i]);
             return;
         }
-        const Tensor st = stats.unpack(), &any = dy.defined() ? dy : dh;
-        const int64_t rows = st.size(0), width = shape.back();
+        const Tensor st = unpack_whole(stats, at::kFloat, {rows, 4}, place, who), &any = dy.defined() ? dy : dh;
         Tensor h[6];
-        for (int i = 0; i < (kept ? 6 : 3); ++i) h[i] = held[i].unpack();
+        if (kept) {
+            for (int i = 0; i < 6; ++i) h[i] = held[i].unpack();
+            for (int i = 0; i < (gated ? 6 : 4); i += 2) {
+                check_kept(h[i], h[i + 1], {rows, width});
+                one_device({&any, &h[i], &h[i + 1]});
+            }
+        } else {
+            for (int i = 0; i < 3; ++i) h[i] = unpack(held[i], at::typeMetaToScalarType(options.dtype()), shape, place, who);
+        }
         const c10::DeviceGuard device(any.device());
         sn_block_norms_args a = norms_args(c, type_of(any), shape, rows);
         a.stats = (float *)pointer(st);
@@ -352,8 +399,9 @@ std::pair<Tensor, Tensor> gated_residual_norms(const Tensor &x, const Tensor &br
         node->stats = SavedVariable(r.stats, false);
         const Tensor given[3] = {x, branch, gate};
         for (int i = 0; i < (kept ? 6 : 3); ++i) node->held[i] = SavedVariable(kept ? r.kept[i] : given[i], false);
-        node->shape = x.sizes().vec();
+        node->shape = at::DimVector(x.sizes());
         node->options = x.options().requires_grad(false);
+        if (first) node->param_type = mixed ? at::kFloat : first->scalar_type();
         node->rms = c.rms, node->eps = c.eps, node->kept = kept, node->gated = gate.defined(), node->empty_rows = !r.stats.defined();
         torch::autograd::set_history(r.y, node);
         if (r.h.defined()) torch::autograd::set_history(r.h, node);
@@ -364,6 +412,8 @@ std::pair<Tensor, Tensor> gated_residual_norms(const Tensor &x, const Tensor &br
 // ------------------------------------------------------------------------------------------------------------------- scores
 struct LabelLogProbsBackward : torch::autograd::Node {
     SavedVariable logits, target, stats;
+    at::DimVector shape;
+    at::TensorOptions options;
     int64_t ignore = 0;
 
     std::string name() const override { return "LabelLogProbsBackward"; }
@@ -381,8 +431,12 @@ struct LabelLogProbsBackward : torch::autograd::Node {
         variable_list out(1);
         if ((grads[0].defined() || grads[1].defined()) && task_should_compute_output(0)) {
             at::AutoDispatchBelowADInplaceOrView raw;
-            const Tensor x = logits.unpack(), t = target.unpack(), s = stats.unpack();
-            const int64_t n = x.size(-1), rows = t.numel();
+            const char *const who = "label_log_probs (backward)";
+            const c10::Device place = options.device();
+            const int64_t n = shape.back(), rows = rows_in(shape);
+            const Tensor x = unpack(logits, at::typeMetaToScalarType(options.dtype()), shape, place, who);
+            const Tensor t = unpack_whole(target, at::kLong, at::IntArrayRef(shape).slice(0, shape.size() - 1), place, who);
+            const Tensor s = unpack_whole(stats, at::kFloat, {rows, 3}, place, who);
             const c10::DeviceGuard device(x.device());
             out[0] = empty(x.sizes(), x, x.scalar_type());
             if (rows) {
@@ -449,6 +503,8 @@ Scores label_log_probs(const Tensor &logits, const Tensor &given, int64_t topk, 
         node->logits = SavedVariable(logits, false);
         node->target = SavedVariable(target, false);
         node->stats = SavedVariable(stats, false);
+        node->shape = at::DimVector(logits.sizes());
+        node->options = logits.options().requires_grad(false);
         node->ignore = ignore;
         torch::autograd::set_history(o.log_probs, node);
         torch::autograd::set_history(o.entropy, node);
@@ -459,26 +515,6 @@ Scores label_log_probs(const Tensor &logits, const Tensor &given, int64_t topk, 
 // ------------------------------------------------------------------------------------------------------- 8-bit checkpoints
 // the entry points' own limits, tested here too: they see the numbers as 32-bit ones
 constexpr int64_t kMostFeatures = 1 << 30, kMostProduct = 1 << 20;
-
-int64_t rows_in(at::IntArrayRef shape)
-{
-    int64_t rows = 1;
-    for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
-    return rows;
-}
-
-// The kernels read codes and exponents by the activation's shape.  Checked at each use: either may have been resized or freed in place
-// since the checkpoint was made, or come back from a hook for saved tensors.
-void check_kept(const Tensor &codes, const Tensor &exps, at::IntArrayRef shape)
-{
-    const int64_t rows = rows_in(shape), npad = (shape.back() + 31) / 32 * 32;
-    auto fits = [&](const Tensor &t, at::ScalarType type, int64_t columns) {
-        return t.defined() && t.scalar_type() == type && t.dim() == 2 && t.size(0) == rows && t.size(1) == columns && t.is_contiguous() &&
-               (int64_t)t.storage().nbytes() >= t.storage_offset() + rows * columns;
-    };
-    if (!fits(codes, at::kChar, npad) || !fits(exps, at::kByte, npad / 32))
-        refuse("checkpoint8: codes and exponents do not hold an activation %s (any more)", shown(shape).c_str());
-}
 
 std::pair<Tensor, Tensor> checkpoint8(const Tensor &x)
 {

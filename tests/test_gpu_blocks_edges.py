@@ -264,3 +264,29 @@ def test_hooks_for_saved_tensors_raise_their_own(ops):
         ops.gated_residual_norms(torch.zeros(1, 4097, device=DEV), torch.zeros(1, 4097, device=DEV))
     with pytest.raises(TypeError):
         ops.gated_residual_norms(x, x, eps="small")
+
+
+@pytest.mark.parametrize("change", [lambda t: t.float() if t.dtype != F32 else t.double(), lambda t: t.cpu(), lambda t: t[..., :1].clone(), lambda t: t.flatten()[:-1].clone(),
+                                    lambda t: t[None].clone()])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_saved_tensors_that_come_back_as_others_are_refused(ops, dtype, change):
+    """hooks that compress or move what is saved and hand back something else: the kernels would read it by the forward call's sizes.  Each
+    saved tensor in turn; the other order of elements is fine"""
+    g = gen(4)
+    x, f, z = (rand(g, 2, 6, 64, dtype=dtype).requires_grad_() for _ in range(3))
+    w = [rand(g, 64, dtype=dtype).requires_grad_() for _ in range(5)]
+    nv, target = torch.tensor([6, 3], dtype=torch.int32, device=DEV), torch.zeros(2, 6, dtype=torch.int64, device=DEV)
+    norms = lambda keep8: ops.gated_residual_norms(x, f, gate=z, scale=w[0], post=(w[1], w[2]), pre=(w[3], w[4]), n_valid=nv, checkpoint8=keep8)[1]      # noqa: E731
+    for call, saved in ((lambda: norms(False), 10), (lambda: norms(True), 13), (lambda: ops.label_log_probs(x, target).log_probs, 3)):
+        for at in range(saved):
+            count = iter(range(100))
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: (next(count), t), lambda p: change(p[1]) if p[0] == at else p[1]):
+                out = call()
+            assert next(count) == saved
+            with pytest.raises(RuntimeError, match="came back as|do not hold|different devices|CUDA tensors"):
+                out.float().sum().backward()
+    for call in (lambda: norms(False), lambda: ops.label_log_probs(x, target).log_probs):
+        want = torch.autograd.grad(call().float().sum(), x)[0]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t.transpose(0, -1).contiguous().transpose(0, -1)):
+            out = call()
+        assert torch.equal(torch.autograd.grad(out.float().sum(), x)[0], want)
