@@ -105,7 +105,14 @@ void check(int rc, const char *what)
 }
 
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-void *pointer(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+// (a NULL pointer tells the library that there is no such tensor: one whose storage was freed must not pass for that)
+void *pointer(const Tensor &t)
+{
+    if (!t.defined()) return nullptr;
+    void *const p = t.data_ptr();
+    if (!p && t.numel()) refuse("a tensor of shape %s has no memory: its storage was freed", shown(t.sizes()).c_str());
+    return p;
+}
 Tensor empty(at::IntArrayRef sizes, const Tensor &like, at::ScalarType type) { return at::empty(sizes, like.options().dtype(type).requires_grad(false)); }
 
 // [..., width]: a tensor that holds the rows (itself where they lie evenly apart, else a copy) and the elements from one row to the next

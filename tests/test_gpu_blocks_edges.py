@@ -1,5 +1,6 @@
 """GPU tests of the operators of include/schemanet_blocks.h at their edges: derivatives that would be lost, values at
-the end of a type's range, gates far open, what a block with 8-bit checkpoints holds in memory, and errors from below."""
+the end of a type's range, gates far open, what a block with 8-bit checkpoints holds in memory, errors from below,
+and tensors of other kinds."""
 import os
 import sys
 
@@ -290,3 +291,36 @@ def test_saved_tensors_that_come_back_as_others_are_refused(ops, dtype, change):
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t.transpose(0, -1).contiguous().transpose(0, -1)):
             out = call()
         assert torch.equal(torch.autograd.grad(out.float().sum(), x)[0], want)
+
+
+# ------------------------------------------------------------------------------------------------ tensors of other kinds
+def message_without(tensor, call):
+    """what `call` raises while the tensor's storage is freed ("": nothing).  The memory is back before anybody can look at the tensor: a
+    failing test prints its arguments, and printing a freed tensor reads address 0."""
+    storage, message = tensor.untyped_storage(), ""
+    size = storage.nbytes()
+    storage.resize_(0)
+    try:
+        call()
+    except RuntimeError as error:
+        message = str(error)
+    finally:
+        storage.resize_(size)
+    return message
+
+
+def test_tensors_without_memory_are_refused(ops):
+    """storages freed to save memory (and not yet filled again): a gate, scale or bias among them must not pass for one that was not given"""
+    g = gen(6)
+    x, f, z = (rand(g, 4, 64) for _ in range(3))
+    w = [rand(g, 64) for _ in range(5)]
+    norms = lambda: ops.gated_residual_norms(x, f, gate=z, scale=w[0], post=(w[1], w[2]), pre=(w[3], w[4]))      # noqa: E731
+    assert all("has no memory" in m for m in [message_without(t, norms) for t in (x, f, z, *w)])
+    target, scale, nv = torch.zeros(4, dtype=torch.int64, device=DEV), w[0].clone().requires_grad_(), torch.ones(2, dtype=torch.int32, device=DEV)
+    y, _ = ops.gated_residual_norms(x, f, scale=scale)
+    kept = ops.checkpoint8(x)
+    messages = [message_without(scale, lambda: y.sum().backward()),
+                message_without(nv, lambda: ops.gated_residual_norms(f.reshape(2, 2, 64), f.reshape(2, 2, 64), n_valid=nv)),
+                message_without(target, lambda: ops.label_log_probs(f, target)), message_without(x, lambda: ops.label_log_probs(x, target)),
+                message_without(x, lambda: ops.checkpoint8(x)), message_without(x, lambda: ops.checkpoint8_weight_grad(x, kept))]
+    assert all("has no memory" in m for m in messages)
