@@ -120,6 +120,7 @@ struct Rows { Tensor t; int64_t stride; };
 Rows rows_of(const Tensor &t, int64_t width)
 {
     if (!t.defined()) return {t, 0};
+    if (t.is_neg()) return {t.resolve_neg().contiguous(), width};           // (a view that stands for its negative, as imag of a conjugate)
     if (t.is_contiguous()) return {t, width};
     if (t.stride(-1) != 1 && width > 1) return {t.contiguous(), width};
     int64_t stride = -1, next = 0;
@@ -386,7 +387,7 @@ std::pair<Tensor, Tensor> gated_residual_norms(const Tensor &x, const Tensor &br
     no_tangents({&x, &branch, &gate, &p[0], &p[1], &p[2], &p[3], &p[4]}, "gated_residual_norms");
     one_device({&x, &branch, &gate, &v, &p[0], &p[1], &p[2], &p[3], &p[4]});
     for (Tensor &t : p)
-        if (t.defined()) t = (mixed ? t.to(at::kFloat) : t).contiguous();
+        if (t.defined()) t = (mixed ? t.to(at::kFloat) : t).resolve_neg().contiguous();
     bool train = false;
     if (at::GradMode::is_enabled()) {
         for (const Tensor *t : {&x, &branch, &gate}) train |= t->defined() && t->requires_grad();
@@ -449,7 +450,7 @@ struct LabelLogProbsBackward : torch::autograd::Node {
             if (rows) {
                 Tensor g[2];
                 for (int i = 0; i < 2; ++i)
-                    if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
+                    if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).resolve_neg().contiguous();
                 const Rows r = rows_of(x, n);
                 check(lib.scores_backward(pointer(r.t), type_of(x), rows, n, r.stride, (const int64_t *)pointer(t), ignore, (const float *)pointer(s),
                                           (const float *)pointer(g[0]), (const float *)pointer(g[1]), pointer(out[0]), stream_of(x)),

@@ -324,3 +324,32 @@ def test_tensors_without_memory_are_refused(ops):
                 message_without(target, lambda: ops.label_log_probs(f, target)), message_without(x, lambda: ops.label_log_probs(x, target)),
                 message_without(x, lambda: ops.checkpoint8(x)), message_without(x, lambda: ops.checkpoint8_weight_grad(x, kept))]
     assert all("has no memory" in m for m in messages)
+
+
+@pytest.mark.parametrize("width", [1, 64])
+def test_negated_views(ops, width):
+    """views that stand for the negative of what lies in memory (imag of a conjugate; with one feature they look contiguous): inputs,
+    parameters and upstream gradients"""
+    g = gen(8)
+    view = lambda *shape: torch._neg_view(rand(g, *shape))      # noqa: E731
+    pair = torch.view_as_complex(rand(g, 6, 1, 2)).conj().imag
+    assert pair.is_neg() and view(3).is_neg() and view(3).is_contiguous()
+    x, f, z = (view(6, width) for _ in range(3)) if width > 1 else (pair, view(6, 1), pair)
+    w = [view(width) for _ in range(5)]
+    norms = lambda x, f, z, w: ops.gated_residual_norms(x, f, gate=z, scale=w[0], post=(w[1], w[2]), pre=(w[3], w[4]))      # noqa: E731
+    real = lambda t: t.resolve_neg().clone()      # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(norms(x, f, z, w), norms(real(x), real(f), real(z), [real(t) for t in w])))
+    kept, plain = ops.checkpoint8(x), ops.checkpoint8(real(x))
+    assert torch.equal(kept.codes, plain.codes) and torch.equal(kept.restore(), plain.restore())
+    assert all(torch.equal(a, b) for a, b in zip(ops.checkpoint8_weight_grad(f, kept), ops.checkpoint8_weight_grad(real(f), kept)))
+    target = torch.zeros(6, dtype=torch.int64, device=DEV)
+    assert all(torch.equal(a, b) for a, b in zip(ops.label_log_probs(x, target, topk=1), ops.label_log_probs(real(x), target, topk=1)))
+    leaf, up, up1 = rand(g, 6, width).requires_grad_(), view(6, width), view(6)
+    for out, u in ((ops.gated_residual_norms(leaf, f)[0], up), (ops.label_log_probs(leaf, target).log_probs, up1), (ops.label_log_probs(leaf, target).entropy, up1)):
+        a, = torch.autograd.grad(out, leaf, u, retain_graph=True)
+        assert torch.equal(a, torch.autograd.grad(out, leaf, real(u))[0])
+    scale = rand(g, width).requires_grad_()
+    y, _ = norms(x, f, z, [torch._neg_view(scale)] + w[1:])
+    a, = torch.autograd.grad(y, scale, up, retain_graph=True)
+    y2, _ = norms(real(x), real(f), real(z), [-scale] + [real(t) for t in w[1:]])
+    assert torch.equal(a, torch.autograd.grad(y2, scale, real(up))[0])
