@@ -186,6 +186,8 @@ class GNN(nn.Module):
     ReLU keeps (its input; a sigmoid its result).  An element of a block, relu / swish: 6.2 / 9.2 bytes, with a gradient for the edges
     9.2 / 12.1, and 20 / 24 without checkpoint8."""
 
+    residual = checkpoint8 = False          # (of modules that were pickled whole before there was a choice)
+
     def __init__(self, num_codes: int, embed_dim: int, num_layers: int, identity_proj: bool = False,
                  activation: str = "relu", residual: bool = False, checkpoint8: bool = False):
         super().__init__()

@@ -1,5 +1,6 @@
 """CPU (-m "not gpu"): calls of the operators of include/schemanet_blocks.h that have to be turned down before a launch: derivatives that
-would be lost, sizes past 32 bits, checkpoints that no longer hold their activation.  No kernel is launched here."""
+would be lost, sizes past 32 bits, checkpoints that no longer hold their activation; and a GNN
+that was pickled before it could be residual.  No kernel is launched here."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -93,3 +94,16 @@ def test_a_checkpoint8_changed_in_place_is_refused(ops, change):
         kept.restore()
     with pytest.raises(RuntimeError, match="do not hold"):
         ops.checkpoint8_weight_grad(torch.zeros(2, 3, 4), kept)
+
+
+def test_a_gnn_pickled_before_it_could_be_residual(ops, tmp_path):
+    """whole modules saved by earlier versions have neither attribute: they are plain ones"""
+    import schema_inference.graph as graph
+    gnn = graph.GNN(10, 32, 2)
+    del gnn.__dict__["residual"], gnn.__dict__["checkpoint8"]
+    torch.save(gnn, tmp_path / "gnn.pt")
+    back = torch.load(tmp_path / "gnn.pt", weights_only=False)
+    assert back.train_folds() is False and back._mfma_ok() and not back.residual and not back.checkpoint8
+    g = torch.Generator().manual_seed(0)
+    nodes, edges, ids = torch.rand(2, 5, generator=g), torch.rand(2, 5, 5, generator=g), torch.randint(0, 10, (2, 5), generator=g)
+    assert torch.equal(back(nodes, edges, ids), graph.GNN.forward(gnn, nodes, edges, ids))
