@@ -3,6 +3,7 @@ stream, raise RuntimeError on a non-zero status.  All tensors are CUDA tensors h
 reference-compatible shims (CPU tensors in, lists out) live in cpp_extension/__init__.py.
 """
 import os
+import weakref
 from ctypes import byref, c_void_p, pointer
 
 import torch
@@ -666,17 +667,27 @@ class Planes:
     k of the blocks (multiple of 16); `scale`: None or a device scalar (fp32 [1], a power of two) - the planes hold
     x * scale."""
 
-    __slots__ = ("hi", "lo", "batches", "rows", "k", "kpad", "scale", "pending", "grad_sum", "compact")
+    __slots__ = ("hi", "lo", "batches", "rows", "k", "kpad", "scale", "edge_sum", "edge_token", "compact")
 
     def __init__(self, hi, lo, batches, rows, k, scale=None):
         self.hi, self.lo, self.batches, self.rows, self.k, self.scale = hi, lo, batches, rows, k, scale
-        self.pending, self.grad_sum = 0, None       # training: products whose backward is still to come / the sum of their dY . X^T
+        self.edge_sum = self.edge_token = None      # training: the _EdgeSum of the products that take this operand / (weak edges, what they take for them)
         self.compact = None                         # training with compacted class graphs: (perm int32 [G, n], n_kept int32 [G]) of an adjacency operand
         self.kpad = (k + 15) // 16 * 16
 
     @property
     def stride(self):
         return self.hi.shape[1] if self.batches > 1 else 0
+
+    @property
+    def pending(self):
+        """training: products whose dY . X^T the present backward pass has summed and not yet handed to the edges"""
+        return self.edge_sum.added if self.edge_sum is not None else 0
+
+    @property
+    def grad_sum(self):
+        """training: that sum"""
+        return self.edge_sum.value if self.edge_sum is not None else None
 
     def to_dense(self):
         """[batches, rows, k] fp32 reconstruction hi + lo (tests / debugging)."""
@@ -984,12 +995,63 @@ class _SymAdjMatmul(torch.autograd.Function):
         return d_adj, d_x, None
 
 
-def _edge_grad_of(s_, adj_planes):
+def _edge_grad_of(s_, compact):
     """S = sum of the layers' dY . X^T -> dE = (S + S^T) / 2; for a compacted operand: its corner symmetrised and scattered back to
     the stored vertex order (zero where a pruned vertex is involved)"""
-    if adj_planes.compact is not None:
-        return sym_scatter_corner(s_, *adj_planes.compact)
+    if compact is not None:
+        return sym_scatter_corner(s_, *compact)
     return sym_half_(s_)
+
+
+class _EdgeSum:
+    """The products of one forward pass share an adjacency operand and the edge tensor: their S = dY . X^T are summed in ONE buffer (the
+    product's epilogue adds) and symmetrised once.  Per layer this was a strided add, a scale and autograd's accumulation: three more
+    passes over a [G, n, n] tensor (404 MB at the ImageNet class graphs' real size).
+    The products take an _EdgeToken in place of the edges.  In each backward pass the first of them to run hands autograd the buffer as the
+    token's gradient, the others add to it and hand over nothing; autograd runs the token's node after all that run in this pass, be it the
+    whole chain, a part of it or the same once more."""
+    __slots__ = ("value", "task", "added")
+
+    def __init__(self):
+        self.take()
+
+    def add(self, product):
+        """product(None) -> a new S, product(S): S += .  -> what the product hands to autograd"""
+        task = torch._C._current_graph_task_id()
+        if task != self.task:                                # (what a pass that did not want the edges' gradient left behind goes)
+            self.value, self.task, self.added = product(None), task, 1
+            return self.value
+        product(self.value)
+        self.added += 1
+        return None
+
+    def take(self):
+        self.value, self.task, self.added = None, -1, 0
+
+
+class _EdgeToken(torch.autograd.Function):
+    """edges [G, n, n] -> a tensor of their shape without memory of its own, float32 whatever their type (a cast of its gradient would part
+    it from the buffer).  ctx holds no operand: operands hold tokens."""
+
+    @staticmethod
+    def forward(ctx, edges, edge_sum, compact):
+        ctx.edge_sum, ctx.compact = edge_sum, compact
+        return torch.empty(1, dtype=torch.float32, device=edges.device).expand(edges.shape)
+
+    @staticmethod
+    def backward(ctx, s_):
+        ctx.edge_sum.take()
+        return _edge_grad_of(s_, ctx.compact), None, None
+
+
+def _shared_edges(edges, adj_planes, sum_edge_grads):
+    """-> what a product takes as its edges, and the sum that its edge gradient goes to (None: to autograd by itself)"""
+    if not (sum_edge_grads and edges.requires_grad and torch.is_grad_enabled() and os.environ.get("SN_GCN_SUM_DE", "1") != "0"):
+        return edges, None
+    if adj_planes.edge_token is None or adj_planes.edge_token[0]() is not edges:
+        adj_planes.edge_sum = _EdgeSum()
+        adj_planes.edge_token = (weakref.ref(edges), _EdgeToken.apply(edges, adj_planes.edge_sum, adj_planes.compact))
+    return adj_planes.edge_token[1], adj_planes.edge_sum
 
 
 class _EdgesAdjMatmul(torch.autograd.Function):
@@ -1000,7 +1062,7 @@ class _EdgesAdjMatmul(torch.autograd.Function):
 
     @staticmethod
     @_amp_fwd
-    def forward(ctx, edges, x, adj_planes, sum_edge_grads=False):
+    def forward(ctx, edges, x, adj_planes, edge_sum=None):
         G = edges.shape[0]
         ext = adj_planes.compact[1] if adj_planes.compact is not None else None      # compacted class graphs: one extent per graph
         xt = split_planes(x.detach(), transpose=True, node_extents=ext)
@@ -1010,9 +1072,7 @@ class _EdgesAdjMatmul(torch.autograd.Function):
         ctx.adj_planes = adj_planes
         ctx.x_scale = xt.scale                               # (the backward's planes of x: no second reduction over it)
         ctx.adj_like = torch.empty(edges.shape, dtype=edges.dtype, device="meta")
-        ctx.counted = bool(sum_edge_grads) and bool(ctx.needs_input_grad[0]) and os.environ.get("SN_GCN_SUM_DE", "1") != "0"
-        if ctx.counted:
-            adj_planes.pending += 1
+        ctx.edge_sum = edge_sum
         return y
 
     @staticmethod
@@ -1033,31 +1093,19 @@ class _EdgesAdjMatmul(torch.autograd.Function):
                            rows_valid=ext)["c"]
         if ctx.needs_input_grad[0]:
             dyp, xp = split_planes(dy, scale=dy_scale, node_extents=ext), split_planes(saved[0].detach(), scale=ctx.x_scale, node_extents=ext)
-            if not ctx.counted:
-                s_ = gcn_gemm(dyp, xp, G, want_c=True, m_extent=ext)["c"]
-                return _edge_grad_of(s_, ap), d_x, None, None
-            # The layers of one forward pass share `ap` and the edge tensor: their S = dY . X^T are summed in ONE buffer (the
-            # product's epilogue adds) and symmetrised once, by the layer whose backward runs last; the others hand autograd
-            # no gradient for the edges (= zero).  Per layer this was a strided add, a scale and autograd's accumulation:
-            # three more passes over a [G, n, n] tensor (404 MB at config [4]'s real size).
-            if ap.grad_sum is None:
-                ap.grad_sum = gcn_gemm(dyp, xp, G, want_c=True, m_extent=ext)["c"]
-            else:
-                gcn_gemm(dyp, xp, G, accumulate_into=ap.grad_sum, m_extent=ext)
-            ap.pending -= 1
-            if ap.pending == 0:
-                d_e, ap.grad_sum = _edge_grad_of(ap.grad_sum, ap), None
+            product = lambda into: gcn_gemm(dyp, xp, G, want_c=into is None, accumulate_into=into, m_extent=ext)["c"]      # noqa: E731
+            d_e = _edge_grad_of(product(None), ap.compact) if ctx.edge_sum is None else ctx.edge_sum.add(product)
         return d_e, d_x, None, None
 
 
 def edges_adj_matmul(edges, x, adj_planes=None, sum_edge_grads=False):
     """edges [G, n, n] fp32, x [G, n, E] fp32 (CUDA, E a multiple of 16) -> ((edges + edges^T)/2 + I) @ x, differentiable in both.
-    sum_edge_grads: the caller applies several of these products IN SEQUENCE to the same `edges` with the same `adj_planes` (the
-    layers of a GNN: every one of them is on the path to the loss if the last is) - their edge gradients are then summed in one
-    buffer and handed to autograd once, by the product whose backward runs last."""
+    sum_edge_grads: the caller applies several of these products to the same `edges` with the same `adj_planes` (the layers of a GNN) -
+    their edge gradients are then summed in one buffer and handed to autograd once in a backward pass."""
     if adj_planes is None:
         adj_planes = gcn_adjacency_planes(edges.detach())
-    return _EdgesAdjMatmul.apply(edges, x, adj_planes, sum_edge_grads)
+    edges, edge_sum = _shared_edges(edges, adj_planes, sum_edge_grads)
+    return _EdgesAdjMatmul.apply(edges, x, adj_planes, edge_sum)
 
 
 def sym_adj_matmul(adj, x, adj_planes=None):
@@ -1162,7 +1210,7 @@ class _GatherAdjMatmul(torch.autograd.Function):
 
     @staticmethod
     @_amp_fwd
-    def forward(ctx, edges, table, ids, bias, adj_planes, sort, padding_idx, sum_edge_grads):
+    def forward(ctx, edges, table, ids, bias, adj_planes, sort, padding_idx, edge_sum):
         G = edges.shape[0]
         tab = _f32c(table.detach())
         t_scale = pow2_scale(tab)
@@ -1173,9 +1221,7 @@ class _GatherAdjMatmul(torch.autograd.Function):
         ctx.adj_planes, ctx.t_scale, ctx.has_bias = adj_planes, t_scale, bias is not None
         ctx.pad = int(padding_idx) if padding_idx is not None else -1
         ctx.adj_like = torch.empty(edges.shape, dtype=edges.dtype, device="meta")
-        ctx.counted = bool(sum_edge_grads) and bool(ctx.needs_input_grad[0]) and os.environ.get("SN_GCN_SUM_DE", "1") != "0"
-        if ctx.counted:
-            adj_planes.pending += 1
+        ctx.edge_sum = edge_sum
         return y
 
     @staticmethod
@@ -1214,16 +1260,8 @@ class _GatherAdjMatmul(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dyp = split_planes(dy, scale=dy_scale, node_extents=ext)
             zp = split_planes(torch.nn.functional.embedding(ids, tab), scale=ctx.t_scale, node_extents=ext)
-            if not ctx.counted:
-                d_e = _edge_grad_of(gcn_gemm(dyp, zp, G, want_c=True, m_extent=ext)["c"], ap)
-            else:
-                if ap.grad_sum is None:
-                    ap.grad_sum = gcn_gemm(dyp, zp, G, want_c=True, m_extent=ext)["c"]
-                else:
-                    gcn_gemm(dyp, zp, G, accumulate_into=ap.grad_sum, m_extent=ext)
-                ap.pending -= 1
-                if ap.pending == 0:
-                    d_e, ap.grad_sum = _edge_grad_of(ap.grad_sum, ap), None
+            product = lambda into: gcn_gemm(dyp, zp, G, want_c=into is None, accumulate_into=into, m_extent=ext)["c"]      # noqa: E731
+            d_e = _edge_grad_of(product(None), ap.compact) if ctx.edge_sum is None else ctx.edge_sum.add(product)
         if ctx.has_bias and ctx.needs_input_grad[3]:
             d_b = dy.sum(dim=(0, 1))
         return d_e, d_tab, None, d_b, None, None, None, None
@@ -1236,7 +1274,8 @@ def gather_adj_matmul(edges, table, ids, bias=None, adj_planes=None, sort=None, 
     sum_edge_grads: as edges_adj_matmul."""
     if adj_planes is None:
         adj_planes = gcn_adjacency_planes(edges.detach())
-    return _GatherAdjMatmul.apply(edges, table, ids.contiguous(), bias, adj_planes, sort, padding_idx, sum_edge_grads)
+    edges, edge_sum = _shared_edges(edges, adj_planes, sum_edge_grads)
+    return _GatherAdjMatmul.apply(edges, table, ids.contiguous(), bias, adj_planes, sort, padding_idx, edge_sum)
 
 
 def pool_fc(pooled_sum, divisor, weight, bias, weight_t=None):

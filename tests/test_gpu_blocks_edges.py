@@ -353,3 +353,76 @@ def test_negated_views(ops, width):
     a, = torch.autograd.grad(y, scale, up, retain_graph=True)
     y2, _ = norms(real(x), real(f), real(z), [-scale] + [real(t) for t in w[1:]])
     assert torch.equal(a, torch.autograd.grad(y2, scale, real(up))[0])
+
+
+# ------------------------------------------------------------------------------------------------ several backward passes over one graph
+@pytest.mark.parametrize("residual,checkpoint8", [(False, False), (True, False), (True, True)])
+@pytest.mark.parametrize("layers", [2, 3])
+def test_several_backward_passes_of_a_gnn(ops, residual, checkpoint8, layers):
+    """a kept graph differentiated again, wholly or for the last layer's parameters only, as programs do that weigh several losses: each pass
+    gives the gradients of a fresh graph, bit for bit.  (The layers sum their products' edge gradients in one buffer.)"""
+    import schema_inference.graph as graph
+    torch.manual_seed(4)
+    kw = dict(residual=True, checkpoint8=checkpoint8) if residual else {}
+    gnn = graph.GNN(50, 64, layers, **kw).to(DEV)
+    data = graphs(n=192, edge_grad=True)
+    data["feat_mask"] = torch.arange(192, device=DEV)[None] >= data["n_valid"][:, None]
+    leaves = [data["edges"]] + list(gnn.parameters())
+    last = [p for p in gnn.layers[-1].parameters()]
+    up = rand(gen(1), 4, 64)
+    fresh = lambda inputs: [t.clone() for t in torch.autograd.grad(gnn(**data), inputs, up)]      # noqa: E731
+    whole, part = fresh(leaves), fresh(last)
+    out = gnn(**data)
+    for inputs, want in ((leaves, whole), (leaves, whole), (last, part), (leaves, whole), (last, part), (last, part), (leaves[:1], whole[:1]), (leaves, whole)):
+        got = torch.autograd.grad(out, inputs, up, retain_graph=True, allow_unused=True)
+        assert all(a is not None and torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("kind", ["gather", "edges"])
+def test_products_of_one_operand_in_parts(ops, kind):
+    """three products in sequence on one edge tensor that autograd reaches in parts: the first two only, the third from a detached input (a
+    backward pass in stages), both at once; the edges' gradient is each time that of products that share nothing"""
+    g = gen(21)
+    G, n, E = 3, 50, 64
+    edges, x = torch.rand(G, n, n, generator=g).to(DEV).requires_grad_(), rand(g, G, n, E).requires_grad_()
+    table, ids = rand(g, 30, E).requires_grad_(), torch.randint(0, 30, (G, n), generator=g).to(DEV)
+    up = rand(g, G, n, E)
+
+    def run(summed):
+        planes = ops.gcn_adjacency_planes(edges.detach())
+        first = (lambda: ops.gather_adj_matmul(edges, table, ids, adj_planes=planes, sum_edge_grads=summed)) if kind == "gather" else (
+            lambda: ops.edges_adj_matmul(edges, x, planes, summed))
+        h1 = first()
+        h2 = ops.edges_adj_matmul(edges, h1.tanh(), planes, summed)
+        cut = h2.detach().requires_grad_()
+        h3 = ops.edges_adj_matmul(edges, cut.tanh(), planes, summed)
+        whole = ops.edges_adj_matmul(edges, h2.tanh(), planes, summed)
+        out = [torch.autograd.grad(h2, edges, up, retain_graph=True)[0]]
+        a, stage = torch.autograd.grad(h3, [edges, cut], up, retain_graph=True)
+        out += [a, torch.autograd.grad(h2, edges, stage, retain_graph=True)[0]]
+        out += [torch.autograd.grad([h3, h2], edges, [up, up], retain_graph=True)[0], torch.autograd.grad(whole, edges, up, retain_graph=True)[0]]
+        torch.autograd.grad(whole, h2, up, retain_graph=True)          # (a pass that does not want the edges)
+        out += [torch.autograd.grad(whole, edges, up)[0]]
+        assert planes.grad_sum is None and planes.pending == 0
+        return out
+    for a, b in zip(run(True), run(False)):
+        # sums of two or three products, symmetrised before or after they are added: a few roundings of the largest
+        assert float((a - b).abs().max()) <= 8 * U * float(b.abs().max())
+
+
+def test_operands_do_not_outlive_their_step(ops):
+    """no cycle keeps an adjacency operand, its edges or the graph alive"""
+    import gc
+    import weakref
+    gc.collect()
+    gc.disable()
+    try:
+        edges, x = rand(gen(1), 2, 40, 40).requires_grad_(), rand(gen(2), 2, 40, 64).requires_grad_()
+        planes = ops.gcn_adjacency_planes(edges.detach())
+        y = ops.edges_adj_matmul(edges, ops.edges_adj_matmul(edges, x, planes, True), planes, True)
+        y.sum().backward()
+        seen = [weakref.ref(t) for t in (planes.hi, planes.edge_token[1], edges)]
+        del planes, y, edges
+        assert [r() for r in seen] == [None, None, None]
+    finally:
+        gc.enable()
