@@ -4,7 +4,8 @@ networks (`gated_residual_norms`), of activations kept in 8 bits for the backwar
 
 They take CUDA tensors in float32, bfloat16 or float16 with rows of any stride, compute in float32 and round each result
 once; outputs are new contiguous tensors; nothing synchronises, all of them can be captured into a graph.  Under `torch.autocast`
-their floating-point inputs are cast to float32, like those of the other HIP-backed ops of this package.  Arguments that do not
+`gated_residual_norms`, `linear_checkpoint8` and `label_log_probs` cast their floating-point inputs to float32, like the other HIP-backed
+ops of this package; `checkpoint8` and `checkpoint8_weight_grad` keep the types that they are given.  Arguments that do not
 fit raise RuntimeError before anything is launched; tensors with a forward-mode tangent, which would be lost, raise
 NotImplementedError.
 

@@ -40,7 +40,8 @@ __global__ __launch_bounds__(kPackThreads) void checkpoint8_kernel(const void *x
 }
 
 // HBM bound: 16 bytes of the result a lane (fp32 32 bytes, 16-bit types 8: slower both at 12544 rows of 256, 4.9 -> 5.4 us and 3.5 -> 4.3, and at
-// 32768 rows of 2048, 69 -> 94 and 31.8 -> 34.3; the latter, bf16, is 6.3 TB/s)
+// 32768 rows of 2048, 69 -> 94 and 31.8 -> 34.3; the same codes again, from the caches).  Codes of their own each time: 6.0 and 3.9 us, 68 and
+// 40; the latter, bf16, is 5.1 TB/s
 template <int DT>
 __global__ __launch_bounds__(kPackThreads) void restore8_kernel(const uint8_t *codes, const uint8_t *exps, int64_t rows, int n, void *out)
 {
@@ -389,8 +390,13 @@ int64_t tiles_of(int out_f, int in_f, int tile) { return (int64_t)((out_f + tile
 
 // Tile and splits of the summed rows.  The large tile where at least 4 of them, times splits, give each of the 256 compute units one
 // with 512 rows or more (32768 rows, bf16: 1024 x 1024 131 us on small tiles, 98 on large ones; 512 x 512 42.0, 41.6; 8192 rows of 512 x 1024
-// 32.0, 37.4), the small one otherwise; then enough splits for two small or one large workgroup on each compute unit (fewer leave
-// units idle, more write partial sums: 1024 x 1024, 512 workgroups of the large tile 117 us, 128 of them 140), at least 256 rows a split
+// 32.0, 37.4), the small one otherwise; then 512 small or 256 large workgroups (fewer leave units idle, more write partial sums: bf16,
+// 1024 x 1024, 512 workgroups of the large tile 117 us, 128 of them 140), at least 256 rows a split.
+// The rule comes from bf16, whose small workgroup takes 64 KB of LDS: two to a compute unit.  fp16's takes 96 KB and fp32's 128, one to a
+// unit: their 512 run in two rounds and write twice the partial sums that 256 would (us with 256 | 512 small workgroups, joining included,
+// bf16, fp16, fp32: 20000 rows of 512 -> 512 30.2 | 29.6, 39.1 | 43.3, 47.7 | 51.7; 8192 of 512 -> 1024 29.0 | 28.6, 35.5 | 39.1, 41.2 | 47.1;
+// 32768 of 256 -> 256 22.2 | 26.0, 25.4 | 32.4, 28.1 | 36.6; 4999 of 387 -> 1000 22.3 | 25.2, 26.3 | 31.3, 29.8 | 34.9; 12544 of 256 -> 256
+// 18.0 | 18.0, 19.8 | 19.6, 22.0 | 21.3).
 struct Split { int tile, n, rows; bool small; };
 Split split_rows(int64_t rows, int out_f, int in_f, int64_t dy_stride)
 {

@@ -263,7 +263,7 @@ __device__ __forceinline__ NormStats statistics(const Row<EV, CH> &r, int col, i
 // the oldest row, the straight lines of the others do not (us, forward / backward, looked up and straight: bf16, 131072 rows of 1024, all
 // parts 268 / 464 and 263 / 408, both norms 253 / 410 and 216 / 312, the second alone 215 / 357 and 191 / 309, the first alone 180 / 327
 // and 141 / 242 (x is not read); 32768 rows of 4096, all parts 326 / 464 and 306 / 418; fp32, 103424 rows of 256, all parts 118 / 162 and
-// 108 / 161).  For the same reason rows that do not count are passed over by scalar arithmetic, and get their zeros in a loop of their own.
+// 108 / 161; with 8-bit checkpoints measured for all parts only: that size padded, backward 145 and 134, bf16 129 and 105).  For the same reason rows that do not count are passed over by scalar arithmetic, and get their zeros in a loop of their own.
 template <int DT, int EV, int CH, bool MULTI, int MODE, bool KEEP>
 __global__ __launch_bounds__(block_of(MULTI)) void norms_forward_kernel(sn_block_norms_args a)
 {
@@ -614,8 +614,10 @@ template <int DT, int EV, int CH, bool MULTI> int launch_forward(const sn_block_
 {
     using L = Layout<DT, EV, CH, MULTI>;
     // Workgroups a compute unit: eight of four waves, eight waves of the wider rows (measured with 1, 2, 3, 4, 8, 16 workgroups: bf16
-    // 131072 x 1024 750 453 311 263 269 280 us; 65536 x 2048 394 275 288 287 286 308; 32768 x 4096 254 271 280 265 266 261; one wave,
-    // fp32 103424 x 256 with 4, 8, 16, 32: 100 109 108 116, bf16 200000 x 256 with 2, 4, 8, 16: 134 106 109 103).
+    // 131072 x 1024 750 453 311 263 269 280 us; 65536 x 2048 394 275 288 287 286 308; 32768 x 4096 254 271 280 265 266 261).  Rows of one
+    // wave, with 2, 4, 6, 8, 16: bf16 200000 x 256 133 111 109 110 107, 200000 x 512 202 208 207 208 205, 12544 x 256 14.4 13.7 13.8 15.1 16.3;
+    // fp32 103424 x 256 125 101 125 110 111, a quarter of it padding 139 104 122 109 104, 103424 x 128 115 76 87 79 79, 12544 x 256 21.7 20.0
+    // 19.4 21.6 22.1: for fp32 four are the better number by 4 to 9 %, eight is what all types take.
     const int W = waves_for(a.width);
     const int64_t turns = (a.rows + L::kRows - 1) / L::kRows, most = 256 * (MULTI ? (8 + W - 1) / W : 8), each = (turns + most - 1) / most;
     using Kernel = void (*)(sn_block_norms_args);

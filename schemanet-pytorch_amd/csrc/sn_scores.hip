@@ -555,7 +555,9 @@ __global__ __launch_bounds__(kScoreThreads) void scores_backward_kernel(ScoreGra
 
 // One wave a row: short rows, and longer ones where there are waves enough (us, wave against workgroup, bf16, without | with 5
 // alternatives: 256 x 2048 4.0, 3.8 | 8.4, 8.1; 256 x 4096 5.0, 3.9 | 13.2, 8.1; 1024 x 4096 5.2, 5.6 | 13.4, 13.1; 2048 x 8192 10.3,
-// 10.6 | 23.7, 28.0; 4096 x 16384 26.5, 28.5 | 50.2, 67.8; 4096 x 32769 49.0, 47.2 | 76.0, 99.8)
+// 10.6 | 23.7, 28.0; 4096 x 16384 26.5, 28.5 | 50.2, 67.8; 4096 x 32769 49.0, 47.2 | 76.0, 99.8; 2048 x 131072 133, 101 | 171, 142).  The rule is
+// made for calls without alternatives: with them many rows of 16385 entries and more, up to somewhere under 131072, would do better by wave,
+// which keeps one list instead of four (4096 x 32769: 76 us, they take 100; with 20 alternatives 109 and 128).
 bool wave_a_row(int64_t rows, int64_t n) { return n <= 2048 || (rows >= 2048 && n <= 16384); }
 // Workgroups a row: one up to 8192 entries (one row of 8192: 3.8 us, in two parts and joined 6.0), else four for each compute unit of
 // 4096 entries or more (16 x 131072, bf16, 20 alternatives: parts of 4096 15.5 us, 8192 16.2, 16384 21.0, 2048 17.9)
