@@ -19,6 +19,7 @@ namespace {
 
 using namespace sn;
 
+constexpr int64_t kMostRows = 1ll << 48;  // (past any memory: sums of a few such numbers stay in 64 bits)
 constexpr int kVectors = 5;              // column sums of the backward pass: pre weight, pre bias, scale, post weight, post bias
 
 // all-reduce over the waves of the workgroup's row (up to 8; the buffers hold zeros for those that are not there); `slot` alternates
@@ -597,7 +598,7 @@ int check_args(const sn_block_norms_args *a, const char *who)
     SN_REQUIRE(a->struct_size == sizeof(sn_block_norms_args), SN_ERR_BAD_ARG, "%s: struct_size %u, the library's is %zu", who, a->struct_size,
                sizeof(sn_block_norms_args));
     SN_REQUIRE(a->dtype >= 0 && a->dtype <= 2 && a->param_dtype >= 0 && a->param_dtype <= 2, SN_ERR_BAD_ARG, "%s: unknown type", who);
-    SN_REQUIRE(a->rows >= 0, SN_ERR_BAD_ARG, "%s: rows %lld", who, (long long)a->rows);
+    SN_REQUIRE(a->rows >= 0 && a->rows <= kMostRows, SN_ERR_BAD_ARG, "%s: rows %lld", who, (long long)a->rows);
     SN_REQUIRE(a->width >= 1 && a->width <= SN_BLOCK_NORMS_MAX_WIDTH, SN_ERR_UNSUPPORTED, "%s: width %d outside 1 .. 4096", who, a->width);
     SN_REQUIRE(!a->n_valid || (a->rows_per_graph > 0 && a->rows % a->rows_per_graph == 0), SN_ERR_BAD_ARG, "%s: rows_per_graph %d", who, a->rows_per_graph);
     SN_REQUIRE((!a->has_post || a->post_weight) && (!a->has_pre || a->pre_weight), SN_ERR_BAD_ARG, "%s: a norm without weight", who);
@@ -683,7 +684,8 @@ extern "C" int sn_block_norms_forward(const sn_block_norms_args *args, void *str
 
 extern "C" size_t sn_block_norms_workspace(int64_t rows, int width)
 {
-    if (rows < 0 || width < 1 || width > SN_BLOCK_NORMS_MAX_WIDTH) return 0;
+    // (no rows: nothing to add up, and no workgroups to divide them among)
+    if (rows < 1 || rows > kMostRows || width < 1 || width > SN_BLOCK_NORMS_MAX_WIDTH) return 0;
     return (size_t)backward_blocks(rows, width) * kVectors * width * sizeof(float);
 }
 

@@ -1,6 +1,10 @@
 """CPU (-m "not gpu"): calls of the operators of include/schemanet_blocks.h that have to be turned down before a launch: derivatives that
-would be lost, sizes past 32 bits, checkpoints that no longer hold their activation; and a GNN
-that was pickled before it could be residual.  No kernel is launched here."""
+would be lost, sizes past 32 bits, checkpoints that no longer hold their activation; a GNN that
+was pickled before it could be residual; and the workspace functions at any numbers.  No kernel is launched here."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -107,3 +111,36 @@ def test_a_gnn_pickled_before_it_could_be_residual(ops, tmp_path):
     g = torch.Generator().manual_seed(0)
     nodes, edges, ids = torch.rand(2, 5, generator=g), torch.rand(2, 5, 5, generator=g), torch.randint(0, 10, (2, 5), generator=g)
     assert torch.equal(back(nodes, edges, ids), graph.GNN.forward(gnn, nodes, edges, ids))
+
+
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "schemanet-pytorch_amd")
+NUMBERS = """
+import itertools, sys
+sys.path.insert(0, sys.argv[1])
+import cpp_extension
+lib = cpp_extension.load()
+rows = (-2**63, -2**31, -1, 0, 1, 2, 63, 64, 2**24 - 1, 2**24, 2**31 - 1, 2**31, 2**32, 2**40, 2**62, 2**63 - 1)
+ints = (-2**31, -1, 0, 1, 31, 32, 33, 128, 256, 4096, 4097, 2**20, 2**20 + 1, 2**30, 2**31 - 1)
+"""
+
+
+def in_a_process(body):
+    """(a division by zero ends the process that makes it)"""
+    done = subprocess.run([sys.executable, "-c", NUMBERS + body, PACKAGE], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, (done.returncode, done.stdout[-300:], done.stderr[-300:])
+
+
+def test_workspace_of_the_norms_at_any_numbers(ops):
+    in_a_process("""
+for r, w in itertools.product(rows, ints):
+    size = lib.sn_block_norms_workspace(r, w)
+    assert (size > 0) == (0 < r <= 2**48 and 1 <= w <= 4096) and size < 2**28, (r, w, size)
+""")
+
+
+def test_workspace_of_the_scores_at_any_numbers(ops):
+    in_a_process("""
+for r, n, k in itertools.product(rows, rows, ints):
+    size = lib.sn_label_log_probs_workspace(r, n, k)
+    assert size == 0 or (0 < r < 1024 and n > 8192 and 0 <= k <= 64 and size <= r * 64 * (4 + 2 * k) * 4), (r, n, k, size)
+""")
