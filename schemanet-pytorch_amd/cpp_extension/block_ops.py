@@ -96,7 +96,8 @@ def checkpoint8(x):
 
 def checkpoint8_weight_grad(dy, kept, bias=True, out_dtype=None):
     """The gradients of y = x W^T + b with respect to W and b from the kept activation: dy [..., out] of float32, bfloat16 or float16,
-    kept = checkpoint8(x) of x [..., in] with the same leading sizes -> (dW [out, in], db [out] or None); in and out up to 2^20.
+    kept = checkpoint8(x) of x [..., in] with the same leading sizes -> (dW [out, in], db [out] or None); in and out up to 2^20,
+    under 2^31 rows.
 
     dW = sum_r dy[r]^T kept[r] on the bf16 matrix cores with float32 sums.  The kept values are exact in bf16 and dy enters as
     bf16 pieces that add up to it (float32: three, float16: two), so the products carry no rounding of their own.  A gradient that is

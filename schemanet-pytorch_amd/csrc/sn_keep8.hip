@@ -13,6 +13,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kPackThreads = 256;
+constexpr int kMostSide = 1 << 20;               // of a weight gradient: features and summed rows
+constexpr int64_t kMostRows = (1ll << 31) - 1;
 
 // HBM bound: one read of x, 1 + 1/32 bytes written per element; a lane holds 8 features, four lanes a block.  32768 rows of 2048, bf16:
 // 36 us, 5.6 TB/s
@@ -488,7 +490,7 @@ extern "C" int sn_checkpoint8_restore(const void *codes, const void *exps, int64
 
 extern "C" size_t sn_checkpoint8_weight_grad_workspace(int64_t rows, int out_features, int in_features, int dy_dtype)
 {
-    if (rows < 0 || out_features < 1 || in_features < 1 || dy_dtype < 0 || dy_dtype > 2) return 0;
+    if (rows < 0 || rows > kMostRows || out_features < 1 || out_features > kMostSide || in_features < 1 || in_features > kMostSide || dy_dtype < 0 || dy_dtype > 2) return 0;
     // (the stride of dy decides between two splits: room for either)
     const int n = split_rows(rows, out_features, in_features, out_features).n, far = split_rows(rows, out_features, in_features, 1 << 22).n;
     const int most = n > far ? n : far;
@@ -501,7 +503,7 @@ extern "C" int sn_checkpoint8_weight_grad(const void *dy, int dy_dtype, int64_t 
     SN_REQUIRE(rows > 0 && out_features >= 1 && in_features >= 1, SN_ERR_BAD_ARG, "sn_checkpoint8_weight_grad: bad rows=%lld out=%d in=%d", (long long)rows,
                out_features, in_features);
     SN_REQUIRE(dy_dtype >= 0 && dy_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, SN_ERR_BAD_ARG, "sn_checkpoint8_weight_grad: unknown type");
-    SN_REQUIRE(out_features <= (1 << 20) && in_features <= (1 << 20) && rows < (1ll << 31), SN_ERR_UNSUPPORTED, "sn_checkpoint8_weight_grad: too large");
+    SN_REQUIRE(out_features <= kMostSide && in_features <= kMostSide && rows <= kMostRows, SN_ERR_UNSUPPORTED, "sn_checkpoint8_weight_grad: too large");
     SN_REQUIRE(dy && codes && exps && dw, SN_ERR_BAD_ARG, "sn_checkpoint8_weight_grad: NULL pointer");
     SN_REQUIRE(workspace && workspace_bytes >= sn_checkpoint8_weight_grad_workspace(rows, out_features, in_features, dy_dtype), SN_ERR_WORKSPACE,
                "sn_checkpoint8_weight_grad: workspace of %zu bytes", workspace_bytes);

@@ -568,6 +568,7 @@ std::pair<Tensor, Tensor> weight_grad(const Tensor &dy, const Tensor &codes, con
         refuse("checkpoint8_weight_grad: gradients %s do not fit the activation %s", shown(dy.sizes()).c_str(), shown(shape).c_str());
     if (dy.size(-1) > kMostProduct || shape.back() > kMostProduct)
         refuse("checkpoint8_weight_grad: %lld x %lld features (at most 2^20 each)", (long long)dy.size(-1), (long long)shape.back());
+    if (rows_in(shape) > INT32_MAX) refuse("checkpoint8_weight_grad: %lld rows (under 2^31)", (long long)rows_in(shape));
     check_kept(codes, exps, shape);
     no_tangents({&dy}, "checkpoint8_weight_grad");
     one_device({&dy, &codes, &exps});

@@ -144,3 +144,21 @@ for r, n, k in itertools.product(rows, rows, ints):
     size = lib.sn_label_log_probs_workspace(r, n, k)
     assert size == 0 or (0 < r < 1024 and n > 8192 and 0 <= k <= 64 and size <= r * 64 * (4 + 2 * k) * 4), (r, n, k, size)
 """)
+
+
+def test_workspace_of_the_weight_gradient_at_any_numbers(ops):
+    in_a_process("""
+for r, o, i, t in itertools.product(rows, ints, ints, (-1, 0, 1, 2, 3)):
+    size = lib.sn_checkpoint8_weight_grad_workspace(r, o, i, t)
+    assert (size > 0) == (0 <= r < 2**31 and 1 <= o <= 2**20 and 1 <= i <= 2**20 and 0 <= t <= 2), (r, o, i, t, size)
+    assert size == 0 or size <= 512 * 4 * (o + 1) * (i + 1) + 16, (r, o, i, t, size)
+""")
+
+
+@pytest.mark.parametrize("rows", [1 << 31, 1 << 32])
+def test_rows_past_32_bits_are_refused(ops, rows):
+    """the workspace of 2^32 rows divided by zero.  (Buffers on the meta device: no memory.)"""
+    codes, exps = torch.empty(rows, 32, dtype=torch.int8, device="meta"), torch.empty(rows, 1, dtype=torch.uint8, device="meta")
+    kept = ops.Checkpoint8(codes, exps, (rows, 7), torch.float32)
+    with pytest.raises(RuntimeError, match="rows"):
+        ops.checkpoint8_weight_grad(torch.zeros(1, 1).expand(rows, 5), kept)
