@@ -426,3 +426,27 @@ def test_operands_do_not_outlive_their_step(ops):
         assert [r() for r in seen] == [None, None, None]
     finally:
         gc.enable()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("keep8", [False, True])
+def test_under_recomputation(ops, reentrant, keep8):
+    """torch's activation checkpointing runs the forward pass again inside the backward pass: the same gradients"""
+    from torch.utils.checkpoint import checkpoint
+    g = gen(31)
+    x, f = rand(g, 3, 10, 64).requires_grad_(), rand(g, 3, 10, 64).requires_grad_()
+    edges, w = torch.rand(3, 10, 10, generator=g).to(DEV).requires_grad_(), rand(g, 64).requires_grad_()
+    target = torch.arange(30, device=DEV).reshape(3, 10)
+
+    def block(x, f, edges, w):
+        planes = ops.gcn_adjacency_planes(edges.detach())
+        y, h = ops.gated_residual_norms(x, ops.edges_adj_matmul(edges, f, planes, True), scale=w, pre=(w, None), checkpoint8=keep8)
+        return ops.label_log_probs(ops.edges_adj_matmul(edges, h, planes, True), target).log_probs + y.sum(-1)
+    results = []
+    for run in (block, lambda *a: checkpoint(block, *a, use_reentrant=reentrant)):
+        for leaf in (x, f, edges, w):
+            leaf.grad = None
+        out = run(x, f, edges, w)
+        out.sum().backward()
+        results.append([out.detach()] + [leaf.grad.clone() for leaf in (x, f, edges, w)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
