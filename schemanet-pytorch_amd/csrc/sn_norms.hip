@@ -74,7 +74,8 @@ template <int DT> __device__ __forceinline__ float sigmoid(float z)
 }
 // The backward pass needs s = sigmoid(z) and 1 - s, each to its own last bits: one register holds the smaller of the two, 1 - s = e s of
 // an open gate (z > 0) as it is, s of a closed one with its sign turned; the other is one subtraction from 1 that cannot cancel.  (1 - s
-// of a rounded s is off by 1e-3 of itself at z = 10 and zero from 17 on.)
+// of a rounded s is off by 1e-3 of itself at z = 10 and zero from 17 on.  13 % more vector instructions in bf16, 8 % in fp32, no time: 32768
+// rows of 4096, bf16, 406 us before and after; 103424 of 256, fp32, padded, from checkpoints, 119 and 120.)
 template <int DT> __device__ __forceinline__ float gate_parts(float z, float &s)
 {
     float e;
