@@ -671,7 +671,7 @@ class Planes:
 
     def __init__(self, hi, lo, batches, rows, k, scale=None):
         self.hi, self.lo, self.batches, self.rows, self.k, self.scale = hi, lo, batches, rows, k, scale
-        self.edge_sum = self.edge_token = None      # training: the _EdgeSum of the products that take this operand / (weak edges, what they take for them)
+        self.edge_sum = self.edge_token = None      # training: the _EdgeSum of the products that take this operand / (the edges, what they take for them), weak
         self.compact = None                         # training with compacted class graphs: (perm int32 [G, n], n_kept int32 [G]) of an adjacency operand
         self.kpad = (k + 15) // 16 * 16
 
@@ -1031,7 +1031,7 @@ class _EdgeSum:
 
 class _EdgeToken(torch.autograd.Function):
     """edges [G, n, n] -> a tensor of their shape without memory of its own, float32 whatever their type (a cast of its gradient would part
-    it from the buffer).  ctx holds no operand: operands hold tokens."""
+    it from the buffer).  ctx holds neither operand nor token."""
 
     @staticmethod
     def forward(ctx, edges, edge_sum, compact):
@@ -1048,10 +1048,15 @@ def _shared_edges(edges, adj_planes, sum_edge_grads):
     """-> what a product takes as its edges, and the sum that its edge gradient goes to (None: to autograd by itself)"""
     if not (sum_edge_grads and edges.requires_grad and torch.is_grad_enabled() and os.environ.get("SN_GCN_SUM_DE", "1") != "0"):
         return edges, None
-    if adj_planes.edge_token is None or adj_planes.edge_token[0]() is not edges:
+    # (the operand refers to the token weakly, the products' nodes keep it: an operand that outlives an eager step must not keep that step's
+    # node of the edges alive, beside which the next step could not be captured)
+    held = adj_planes.edge_token
+    token = held[1]() if held is not None and held[0]() is edges else None
+    if token is None:
         adj_planes.edge_sum = _EdgeSum()
-        adj_planes.edge_token = (weakref.ref(edges), _EdgeToken.apply(edges, adj_planes.edge_sum, adj_planes.compact))
-    return adj_planes.edge_token[1], adj_planes.edge_sum
+        token = _EdgeToken.apply(edges, adj_planes.edge_sum, adj_planes.compact)
+        adj_planes.edge_token = weakref.ref(edges), weakref.ref(token)
+    return token, adj_planes.edge_sum
 
 
 class _EdgesAdjMatmul(torch.autograd.Function):
@@ -1072,7 +1077,7 @@ class _EdgesAdjMatmul(torch.autograd.Function):
         ctx.adj_planes = adj_planes
         ctx.x_scale = xt.scale                               # (the backward's planes of x: no second reduction over it)
         ctx.adj_like = torch.empty(edges.shape, dtype=edges.dtype, device="meta")
-        ctx.edge_sum = edge_sum
+        ctx.edge_sum, ctx.token = edge_sum, edges if edge_sum is not None else None
         return y
 
     @staticmethod
@@ -1221,7 +1226,7 @@ class _GatherAdjMatmul(torch.autograd.Function):
         ctx.adj_planes, ctx.t_scale, ctx.has_bias = adj_planes, t_scale, bias is not None
         ctx.pad = int(padding_idx) if padding_idx is not None else -1
         ctx.adj_like = torch.empty(edges.shape, dtype=edges.dtype, device="meta")
-        ctx.edge_sum = edge_sum
+        ctx.edge_sum, ctx.token = edge_sum, edges if edge_sum is not None else None
         return y
 
     @staticmethod

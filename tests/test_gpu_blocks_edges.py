@@ -421,9 +421,12 @@ def test_operands_do_not_outlive_their_step(ops):
         planes = ops.gcn_adjacency_planes(edges.detach())
         y = ops.edges_adj_matmul(edges, ops.edges_adj_matmul(edges, x, planes, True), planes, True)
         y.sum().backward()
-        seen = [weakref.ref(t) for t in (planes.hi, planes.edge_token[1], edges)]
-        del planes, y, edges
-        assert [r() for r in seen] == [None, None, None]
+        assert planes.edge_token[1]() is not None
+        del y
+        assert planes.edge_token[1]() is None                          # (the graph is gone, the operand keeps nothing of it)
+        seen = [weakref.ref(t) for t in (planes.hi, edges)]
+        del planes, edges
+        assert [r() for r in seen] == [None, None]
     finally:
         gc.enable()
 
@@ -450,3 +453,34 @@ def test_under_recomputation(ops, reentrant, keep8):
         out.sum().backward()
         results.append([out.detach()] + [leaf.grad.clone() for leaf in (x, f, edges, w)])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_an_operand_used_for_several_steps(ops):
+    """the adjacency operand of edges that stay the same: eager steps one after the other, on another stream, and captured, each with the
+    gradients of an operand of its own"""
+    g = gen(41)
+    edges, x, up = torch.rand(2, 40, 40, generator=g).to(DEV).requires_grad_(), rand(g, 2, 40, 64).requires_grad_(), rand(g, 2, 40, 64)
+
+    def step(planes):
+        y = ops.edges_adj_matmul(edges, ops.edges_adj_matmul(edges, x, planes, True).tanh(), planes, True)
+        return torch.autograd.grad(y, [edges, x], up)
+    want = [t.clone() for t in step(ops.gcn_adjacency_planes(edges.detach()))]
+    same = lambda got: all(torch.equal(a, b) for a, b in zip(got, want))      # noqa: E731
+    planes = ops.gcn_adjacency_planes(edges.detach())
+    assert same(step(planes)) and same(step(planes))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(planes)
+    torch.cuda.current_stream().wait_stream(side)
+    assert same(got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(planes)
+    for _ in range(3):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out)
+    assert same(step(planes))
